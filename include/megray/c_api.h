@@ -182,6 +182,54 @@ int megray_add_rmsnorm_bf16(const void* x, const void* y, void* x_out, void* n_o
 int megray_rmsnorm_bwd_bf16(const void* dn, const void* n, const float* inv_rms, const void* dres,
                             void* dx, int rows, int cols, void* stream);
 
+/* AdamW over a list of tensors.  `block` is the tensor's first block of 256 elements in the moment buffers,
+ * which cover whole blocks.  bits = 32: m and v are float32; bits = 8: m and v hold e4m3 numbers of m and of
+ * sqrt(v), the scales one float32 per block.  The *_dev pointers, where not null, name one float32 on the device each
+ * that takes the place of the host value (a captured graph then follows them). */
+typedef struct {
+    void* p;
+    const void* g;
+    void* copy;          /* bf16 copy of the updated parameters, or null */
+    uint64_t n, block;
+} megray_adamw_tensor;
+typedef struct {
+    int p_dtype, g_dtype, bits;   /* MEGRAY_FLOAT32 or MEGRAY_BFLOAT16 */
+    void *m, *v;
+    float *m_scale, *v_scale;
+    double lr, beta1, beta2, eps, weight_decay, grad_scale, step;
+    const float *lr_dev, *grad_scale_dev, *step_dev;
+} megray_adamw_args;
+int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_adamw_args* args, void* stream);
+
+/* Balance loss of a router (src/kernels/balance.cuh): loss = coef * experts * sum_e f[e] P[e] with the share f of
+ * the counted pairs and the mean probability P of every expert, pairs per expert, and the gradient of the logits.
+ * megray_balance makes at most two launches; `workspace` holds megray_balance_workspace(tokens, experts) bytes.  The two
+ * halves apart, for partial sums that are added up over ranks in between: megray_balance_stats writes
+ * megray_balance_partials(tokens, experts) records of megray_balance_record(experts) bytes (float sums[experts], int32
+ * counts[experts], int32 tokens), megray_balance_grad reads `n_partials` of them. */
+typedef struct {
+    const void* logits;    /* [tokens, experts], rows `ld` elements apart */
+    const void* idx;       /* [tokens, top] contiguous; entries outside [0, experts) are not counted */
+    const uint8_t* mask;   /* [tokens], 0 = the token does not count; or null */
+    int64_t ld;
+    int dtype, idx64;      /* MEGRAY_FLOAT32 or MEGRAY_BFLOAT16; idx is int64 instead of int32 */
+    int tokens, experts, top;
+} megray_router;
+typedef struct {
+    float* loss;
+    int* counts;
+    void* dlogits;         /* or null; rows `ldd` elements apart */
+    int64_t ldd;
+    int dtype, accumulate; /* the logits' type or MEGRAY_FLOAT32; add to what dlogits holds */
+    float coef;
+} megray_balance_out;
+size_t megray_balance_workspace(int tokens, int experts);
+int megray_balance_partials(int tokens, int experts);
+size_t megray_balance_record(int experts);
+int megray_balance_stats(const megray_router* r, void* partials, void* stream);
+int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const megray_balance_out* out, void* stream);
+int megray_balance(const megray_router* r, const megray_balance_out* out, void* workspace, void* stream);
+
 /* ---- one pass of the single-GPU models -----------------------------------------------------------
  * The launches of megray_b200/models (tp_mlp.py, moe.py without a communicator) as one call each.
  * All matrices are contiguous bf16, row-major; nothing is kept between calls. */

@@ -82,6 +82,29 @@ class MoEArgs(C.Structure):
                   "block_group", "total", "w", "dw", "dlogits", "error_flag")])
 
 
+class AdamWArgs(C.Structure):
+    """Mirror of ``megray_adamw_args``."""
+
+    _fields_ = ([(n, C.c_int) for n in ("p_dtype", "g_dtype", "bits")] +
+                [(n, C.c_void_p) for n in ("m", "v", "m_scale", "v_scale")] +
+                [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale", "step")] +
+                [(n, C.c_void_p) for n in ("lr_dev", "grad_scale_dev", "step_dev")])
+
+
+class Router(C.Structure):
+    """Mirror of ``megray_router``."""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("logits", "idx", "mask")] + [("ld", C.c_int64)] +
+                [(n, C.c_int) for n in ("dtype", "idx64", "tokens", "experts", "top")])
+
+
+class BalanceOut(C.Structure):
+    """Mirror of ``megray_balance_out``."""
+
+    _fields_ = ([(n, C.c_void_p) for n in ("loss", "counts", "dlogits")] + [("ldd", C.c_int64)] +
+                [(n, C.c_int) for n in ("dtype", "accumulate")] + [("coef", C.c_float)])
+
+
 def _declare(lib) -> None:
     """argtypes / restype of the C interface (include/megray/c_api.h)."""
     vp, u32, u64, i32, i64, sz = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_int64, C.c_size_t
@@ -153,6 +176,13 @@ def _declare(lib) -> None:
     d("megray_mse_bf16", i32, vp, vp, vp, vp, u64, C.c_float, vp)
     d("megray_add_rmsnorm_bf16", i32, vp, vp, vp, vp, vp, i32, i32, C.c_float, vp)
     d("megray_rmsnorm_bwd_bf16", i32, vp, vp, vp, vp, vp, i32, i32, vp)
+    d("megray_adamw", i32, vp, i32, P(AdamWArgs), vp)
+    d("megray_balance_workspace", sz, i32, i32)
+    d("megray_balance_partials", i32, i32, i32)
+    d("megray_balance_record", sz, i32)
+    d("megray_balance_stats", i32, P(Router), vp, vp)
+    d("megray_balance_grad", i32, P(Router), vp, i32, P(BalanceOut), vp)
+    d("megray_balance", i32, P(Router), P(BalanceOut), vp, vp)
     d("megray_tp_ag_gemm", i32, vp, P(GemmArgs), vp, vp, vp, vp)
     d("megray_tp_gemm_rs", i32, vp, P(GemmArgs), vp, vp, vp, vp, C.c_size_t, vp)
     d("megray_tp_rs_counter_bytes", C.c_size_t, i32, i32)

@@ -1,0 +1,89 @@
+// C entry points of the transformer training operators (see include/megray/c_api.h).
+#include "kernels/adamw.cuh"
+#include "kernels/balance.cuh"
+#include "megray/c_api.h"
+#include "megray/types.h"
+
+namespace {
+constexpr int kInvalid = 6;
+int rc(cudaError_t e) { return e == cudaSuccess ? 0 : -static_cast<int>(e); }
+cudaStream_t S(void* s) { return static_cast<cudaStream_t>(s); }
+bool f32_or_bf16(int dtype) { return dtype == MegRay::MEGRAY_FLOAT32 || dtype == MegRay::MEGRAY_BFLOAT16; }
+bool is_bf16(int dtype) { return dtype == MegRay::MEGRAY_BFLOAT16; }
+
+bool to_router(const megray_router* r, mgk::balance::Router* to) {
+    if (r == nullptr || !f32_or_bf16(r->dtype))
+        return false;
+    *to = {r->logits, is_bf16(r->dtype), r->ld, r->idx, r->idx64 != 0, r->mask, r->tokens, r->experts, r->top};
+    return true;
+}
+bool to_result(const megray_balance_out* o, mgk::balance::Result* to) {
+    if (o == nullptr || (o->dlogits != nullptr && !f32_or_bf16(o->dtype)))
+        return false;
+    *to = {o->coef, o->loss, o->counts, o->dlogits, is_bf16(o->dtype), o->ldd, o->accumulate != 0};
+    return true;
+}
+}  // namespace
+
+extern "C" {
+
+int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_adamw_args* a, void* stream) {
+    if (a == nullptr || !f32_or_bf16(a->p_dtype) || !f32_or_bf16(a->g_dtype))
+        return kInvalid;
+    static_assert(sizeof(megray_adamw_tensor) == sizeof(mgk::adamw::Tensor), "the list is passed on as it is");
+    mgk::adamw::Step s{};
+    s.p_bf16 = is_bf16(a->p_dtype);
+    s.g_bf16 = is_bf16(a->g_dtype);
+    s.bits = a->bits;
+    s.m = a->m;
+    s.v = a->v;
+    s.m_scale = a->m_scale;
+    s.v_scale = a->v_scale;
+    s.lr = a->lr;
+    s.beta1 = a->beta1;
+    s.beta2 = a->beta2;
+    s.eps = a->eps;
+    s.weight_decay = a->weight_decay;
+    s.grad_scale = a->grad_scale;
+    s.step = a->step;
+    s.lr_dev = a->lr_dev;
+    s.grad_scale_dev = a->grad_scale_dev;
+    s.step_dev = a->step_dev;
+    return rc(mgk::adamw::launch(reinterpret_cast<const mgk::adamw::Tensor*>(tensors), count, s, S(stream)));
+}
+
+int megray_balance_partials(int tokens, int experts) { return mgk::balance::partials(tokens, experts); }
+size_t megray_balance_record(int experts) { return static_cast<size_t>(mgk::balance::partial_words(experts)) * 4; }
+size_t megray_balance_workspace(int tokens, int experts) {
+    return mgk::balance::partials(tokens, experts) * megray_balance_record(experts);
+}
+int megray_balance_stats(const megray_router* r, void* partials, void* stream) {
+    mgk::balance::Router router;
+    if (!to_router(r, &router))
+        return kInvalid;
+    return rc(mgk::balance::launch_stats(router, partials, S(stream)));
+}
+int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const megray_balance_out* out,
+                        void* stream) {
+    mgk::balance::Router router;
+    mgk::balance::Result result;
+    if (!to_router(r, &router) || !to_result(out, &result))
+        return kInvalid;
+    return rc(mgk::balance::launch_grad(router, partials, n_partials, result, S(stream)));
+}
+int megray_balance(const megray_router* r, const megray_balance_out* out, void* workspace, void* stream) {
+    mgk::balance::Router router;
+    mgk::balance::Result result;
+    if (!to_router(r, &router) || !to_result(out, &result))
+        return kInvalid;
+    const cudaError_t one = mgk::balance::launch_small(router, result, S(stream));
+    if (one != cudaErrorNotSupported)
+        return rc(one);
+    const cudaError_t e = mgk::balance::launch_stats(router, workspace, S(stream));
+    if (e != cudaSuccess)
+        return rc(e);
+    return rc(mgk::balance::launch_grad(router, workspace, mgk::balance::partials(router.tokens, router.experts), result,
+                                        S(stream)));
+}
+
+}  // extern "C"
