@@ -182,6 +182,28 @@ int megray_add_rmsnorm_bf16(const void* x, const void* y, void* x_out, void* n_o
 int megray_rmsnorm_bwd_bf16(const void* dn, const void* n, const float* inv_rms, const void* dres,
                             void* dx, int rows, int cols, void* stream);
 
+/* Softmax attention over prompts that are packed one behind the other (src/kernels/attention.cuh).  Tensors are [tokens,
+ * heads, dim] with strides in elements, multiples of 8, the innermost contiguous, 16-byte aligned.  Sequence s holds rows
+ * cu[s] .. cu[s + 1] (device array of seqs + 1); without cu all rows are one.  Rows behind the last sequence are neither
+ * used nor written.  lse is [heads, tokens]; `delta` a workspace of heads * tokens floats. */
+typedef struct {
+    void* p;
+    int64_t row, head;
+} megray_attn_tensor;
+typedef struct {
+    const int* cu;
+    int dtype;            /* MEGRAY_BFLOAT16 or MEGRAY_FLOAT16 */
+    int tokens, heads, kv_heads, dim, seqs, causal;
+    float scale;
+    int* error_flag;      /* device word, set to 1 when a wait inside a kernel runs out; or null */
+} megray_attn_args;
+int megray_attention(const megray_attn_args* a, const megray_attn_tensor* q, const megray_attn_tensor* k,
+                     const megray_attn_tensor* v, const megray_attn_tensor* out, float* lse, void* stream);
+int megray_attention_bwd(const megray_attn_args* a, const megray_attn_tensor* dout, const megray_attn_tensor* q,
+                         const megray_attn_tensor* k, const megray_attn_tensor* v, const megray_attn_tensor* out,
+                         const float* lse, const megray_attn_tensor* dq, const megray_attn_tensor* dk,
+                         const megray_attn_tensor* dv, float* delta, void* stream);
+
 /* AdamW over a list of tensors.  `block` is the tensor's first block of 256 elements in the moment buffers,
  * which cover whole blocks.  bits = 32: m and v are float32; bits = 8: m and v hold e4m3 numbers of m and of
  * sqrt(v), the scales one float32 per block.  The *_dev pointers, where not null, name one float32 on the device each

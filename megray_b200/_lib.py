@@ -82,6 +82,20 @@ class MoEArgs(C.Structure):
                   "block_group", "total", "w", "dw", "dlogits", "error_flag")])
 
 
+class AttnTensor(C.Structure):
+    """Mirror of ``megray_attn_tensor``."""
+
+    _fields_ = [("p", C.c_void_p), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class AttnArgs(C.Structure):
+    """Mirror of ``megray_attn_args``."""
+
+    _fields_ = ([("cu", C.c_void_p)] +
+                [(n, C.c_int) for n in ("dtype", "tokens", "heads", "kv_heads", "dim", "seqs", "causal")] +
+                [("scale", C.c_float), ("error_flag", C.c_void_p)])
+
+
 class AdamWArgs(C.Structure):
     """Mirror of ``megray_adamw_args``."""
 
@@ -176,6 +190,9 @@ def _declare(lib) -> None:
     d("megray_mse_bf16", i32, vp, vp, vp, vp, u64, C.c_float, vp)
     d("megray_add_rmsnorm_bf16", i32, vp, vp, vp, vp, vp, i32, i32, C.c_float, vp)
     d("megray_rmsnorm_bwd_bf16", i32, vp, vp, vp, vp, vp, i32, i32, vp)
+    at = P(AttnTensor)
+    d("megray_attention", i32, P(AttnArgs), at, at, at, at, vp, vp)
+    d("megray_attention_bwd", i32, P(AttnArgs), at, at, at, at, at, vp, at, at, at, vp, vp)
     d("megray_adamw", i32, vp, i32, P(AdamWArgs), vp)
     d("megray_balance_workspace", sz, i32, i32)
     d("megray_balance_partials", i32, i32, i32)

@@ -1,0 +1,129 @@
+"""Softmax attention over whole prompts and its backward pass (src/kernels/attention.cu).
+
+Prompts lie one behind the other in the rows of ``[T, heads, D]`` tensors; ``cu_seqlens`` (int32, on the device,
+``[0, L0, L0 + L1, ...]``) says where each begins.  A query sees the keys of its own prompt, with ``causal`` those up to
+its own position.  Key / value heads may be fewer than query heads: query head h reads key / value head
+``h * Hk // H``.  bf16 or float16, D a multiple of 8 up to 128, any strides that are multiples of 8 elements
+(slices of one projection among them).
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from .. import _lib
+from ._stream import raw_stream
+from .gemm import gemm_error_flag
+
+_CODES = {torch.float16: 6, torch.bfloat16: 10}
+
+
+def _tensor(t: torch.Tensor, shape, like: torch.Tensor, name: str):
+    """The C view of a [T, heads, D] tensor; ValueError for anything that the kernels do not read."""
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise ValueError(f"attention: {name} is a {tuple(shape)} {like.dtype} tensor on the queries' device")
+    rows, heads, dim = shape
+    # the stride of an axis of one is never used
+    head = t.stride(1) if heads > 1 else dim
+    row = t.stride(0) if rows > 1 else max(8, heads * head)
+    if rows and (t.stride(2) != 1 or row % 8 or head % 8 or row <= 0 or head <= 0 or t.data_ptr() % 16):
+        raise ValueError(f"attention: {name}: innermost axis contiguous, the other strides multiples of 8 elements, "
+                         "16-byte aligned")
+    return _lib.AttnTensor(t.data_ptr() or None, row, head)
+
+
+def _output(t, shape, like: torch.Tensor, name: str):
+    t = torch.empty(shape, dtype=like.dtype, device=like.device) if t is None else t
+    c = _tensor(t, shape, like, name)
+    rows, heads, dim = shape
+    # (token by token or head by head, every element has an address of its own)
+    if rows > 1 and heads > 1 and not (c.head >= dim and c.row >= heads * c.head - (c.head - dim) or
+                                       c.row >= dim and c.head >= rows * c.row - (c.row - dim)) or \
+            (rows > 1 and c.row < dim):
+        raise ValueError(f"attention: {name} overlaps itself")
+    return t, c
+
+
+def _problem(q, k, v, cu_seqlens, causal, scale):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.is_cuda or q.dtype not in _CODES:
+        raise ValueError("attention: q is a [T, heads, D] CUDA tensor, bf16 or float16")
+    tokens, heads, dim = q.shape
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("attention: k is a [T, kv heads, D] tensor")
+    kv_heads = k.shape[1]
+    if dim % 8 or not 8 <= dim <= 128 or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError("attention: D is a multiple of 8 from 8 to 128, the query heads a multiple of the key heads")
+    if scale is None:
+        scale = 1.0 / math.sqrt(dim)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("attention: scale is positive")
+    cu, seqs = None, 1
+    if cu_seqlens is not None:
+        if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or
+                not cu_seqlens.is_contiguous() or cu_seqlens.device != q.device):
+            raise ValueError("attention: cu_seqlens is a contiguous int32 tensor of at least 2 entries on q's device")
+        cu, seqs = cu_seqlens.data_ptr(), cu_seqlens.numel() - 1
+    args = _lib.AttnArgs(cu, _CODES[q.dtype], tokens, heads, kv_heads, dim, seqs, int(bool(causal)), scale,
+                         gemm_error_flag(q.device).data_ptr())
+    kv = (tokens, kv_heads, dim)
+    return args, _tensor(q, q.shape, q, "q"), _tensor(k, kv, q, "k"), _tensor(v, kv, q, "v")
+
+
+def _row_sums(t, heads: int, tokens: int, like: torch.Tensor, name: str) -> torch.Tensor:
+    if t is None:
+        return torch.empty(heads, tokens, dtype=torch.float32, device=like.device)
+    if t.dtype != torch.float32 or t.shape != (heads, tokens) or not t.is_contiguous() or t.device != like.device:
+        raise ValueError(f"attention: {name} is a contiguous [heads, T] float32 tensor on the queries' device")
+    return t
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor = None, *, causal: bool = True,
+              scale: float = None, out: torch.Tensor = None, lse: torch.Tensor = None):
+    """Returns (out, lse): out = softmax(scale * q k^T) v in the type of ``q`` (``[T, H, D]``) and the logarithm of the
+    sum of exponentials of every row (``[H, T]`` float32), which the backward pass takes and with which results
+    over several sets of keys are joined.  ``scale`` defaults to 1 / sqrt(D).
+
+    Without ``cu_seqlens`` all rows are one prompt.  Rows behind the last prompt are not looked at and keep what
+    ``out`` and ``lse`` hold there (undefined in tensors made here).  ``cu_seqlens`` is read on the device: it has to
+    rise from 0 to at most T; nothing outside the tensors is touched if it does not, but rows may then go
+    unwritten.  Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32.  A NaN or
+    an infinity in the values of a prompt may reach any row of that prompt, those of other prompts and of rows
+    behind the last never do."""
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return attention(q, k, v, cu_seqlens, causal=causal, scale=scale, out=out, lse=lse)
+    args, cq, ck, cv = _problem(q, k, v, cu_seqlens, causal, scale)
+    out, co = _output(out, q.shape, q, "out")
+    lse = _row_sums(lse, q.shape[1], q.shape[0], q, "lse")
+    rc = _lib.load().megray_attention(args, cq, ck, cv, co, lse.data_ptr(), raw_stream())
+    if rc != 0:
+        raise RuntimeError(f"megray_attention failed ({rc})")
+    return out, lse
+
+
+def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                  lse: torch.Tensor, cu_seqlens: torch.Tensor = None, *, causal: bool = True, scale: float = None,
+                  dq: torch.Tensor = None, dk: torch.Tensor = None, dv: torch.Tensor = None):
+    """Returns (dq, dk, dv) for the gradient ``dout`` of the ``out`` that :func:`attention` returned with ``lse`` for the
+    same arguments.  Gradients of key / value heads are summed over the query heads that read them.  Given tensors
+    are written to (any of the strides that the inputs may have, slices of one buffer among them); rows behind the
+    last prompt are left as they are.  No atomics: the same inputs give the same bits."""
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return attention_bwd(dout, q, k, v, out, lse, cu_seqlens, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)
+    args, cq, ck, cv = _problem(q, k, v, cu_seqlens, causal, scale)
+    tokens, heads, _ = q.shape
+    co, cd = _tensor(out, q.shape, q, "out"), _tensor(dout, q.shape, q, "dout")
+    if lse is None:
+        raise ValueError("attention_bwd: lse is what attention returned")
+    lse = _row_sums(lse, heads, tokens, q, "lse")
+    dq, cdq = _output(dq, q.shape, q, "dq")
+    dk, cdk = _output(dk, k.shape, q, "dk")
+    dv, cdv = _output(dv, k.shape, q, "dv")
+    delta = torch.empty(heads, tokens, dtype=torch.float32, device=q.device)
+    rc = _lib.load().megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, delta.data_ptr(),
+                                          raw_stream())
+    if rc != 0:
+        raise RuntimeError(f"megray_attention_bwd failed ({rc})")
+    return dq, dk, dv

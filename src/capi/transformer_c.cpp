@@ -1,5 +1,6 @@
 // C entry points of the transformer training operators (see include/megray/c_api.h).
 #include "kernels/adamw.cuh"
+#include "kernels/attention.cuh"
 #include "kernels/balance.cuh"
 #include "megray/c_api.h"
 #include "megray/types.h"
@@ -23,9 +24,36 @@ bool to_result(const megray_balance_out* o, mgk::balance::Result* to) {
     *to = {o->coef, o->loss, o->counts, o->dlogits, is_bf16(o->dtype), o->ldd, o->accumulate != 0};
     return true;
 }
+bool to_problem(const megray_attn_args* a, mgk::attn::Problem* to) {
+    if (a == nullptr || (a->dtype != MegRay::MEGRAY_BFLOAT16 && a->dtype != MegRay::MEGRAY_FLOAT16))
+        return false;
+    *to = {a->dtype == MegRay::MEGRAY_FLOAT16, a->tokens, a->heads, a->kv_heads, a->dim, a->cu, a->seqs,
+           a->causal != 0, a->scale, a->error_flag};
+    return true;
+}
+mgk::attn::Tensor T(const megray_attn_tensor* t) {
+    return t != nullptr ? mgk::attn::Tensor{t->p, t->row, t->head} : mgk::attn::Tensor{};
+}
 }  // namespace
 
 extern "C" {
+
+int megray_attention(const megray_attn_args* a, const megray_attn_tensor* q, const megray_attn_tensor* k,
+                     const megray_attn_tensor* v, const megray_attn_tensor* out, float* lse, void* stream) {
+    mgk::attn::Problem p;
+    if (!to_problem(a, &p))
+        return kInvalid;
+    return rc(mgk::attn::launch_forward(p, T(q), T(k), T(v), T(out), lse, S(stream)));
+}
+int megray_attention_bwd(const megray_attn_args* a, const megray_attn_tensor* dout, const megray_attn_tensor* q,
+                         const megray_attn_tensor* k, const megray_attn_tensor* v, const megray_attn_tensor* out,
+                         const float* lse, const megray_attn_tensor* dq, const megray_attn_tensor* dk,
+                         const megray_attn_tensor* dv, float* delta, void* stream) {
+    mgk::attn::Problem p;
+    if (!to_problem(a, &p))
+        return kInvalid;
+    return rc(mgk::attn::launch_backward(p, T(dout), T(q), T(k), T(v), T(out), lse, T(dq), T(dk), T(dv), delta, S(stream)));
+}
 
 int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_adamw_args* a, void* stream) {
     if (a == nullptr || !f32_or_bf16(a->p_dtype) || !f32_or_bf16(a->g_dtype))

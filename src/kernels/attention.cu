@@ -1,0 +1,1113 @@
+// Attention over packed prompts on the tensor cores:
+//
+//   S = scale Q K^T (masked)   P = exp(S - lse)   O = P V          lse = log sum exp S, row by row
+//   delta = rowsum(O * dO)     dV = P^T dO        dS = P * (dO V^T - delta)
+//   dQ = scale dS K            dK = scale dS^T Q  (dK and dV summed over the query heads of a group)
+//
+// Three kernels of one shape: a TMA warp, a warp whose elected lane issues every tcgen05.mma, and two warpgroups
+// that turn scores into probabilities, one thread a row (a TMEM lane).  Tiles are 128 rows of 64 (dim <= 64) or
+// 128 elements in 128-byte-swizzled shared memory; a dimension in between is filled up with zeros by TMA, and the
+// products run over the multiple of 16 that covers it.  P and dS are the products' left operands straight from
+// TMEM: they are written over the scores they come from, as 16-bit pairs, and never pass through shared memory.
+// That rounding to 16 bits is the one the operands of the tensor cores ask for; sums, maxima, lse, delta and the
+// accumulators are float32.
+//
+// Rows of other sequences.  The tile at a sequence's end also holds rows of the next one or of padding.  Scores of
+// such keys are replaced, not added to; but a probability of zero times a NaN in such a row would reach the sum, so
+// the rows that a product sums over are zeroed in shared memory behind the sequence's end.
+//
+// Backward without atomics: dQ in a kernel of its own (one tile of queries, all keys) beside dK and dV (one tile of
+// keys, all queries of all heads of the group).  S and dO V^T are formed twice, seven products instead of five, and
+// in return no float32 sums of dQ go through memory and the same bits come out every time.
+#include "attention.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "gemm_device.cuh"
+#include "launch_count.h"
+
+namespace mgk {
+namespace attn {
+
+namespace {
+
+using namespace mgk::ptx;
+
+constexpr int TILE = 128;
+constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 elements
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr uint64_t WAIT_NS = 4000000000ull;
+
+struct Params {
+    const int* cu;
+    int seqs, tokens, heads, kv_heads, dim;
+    int causal;
+    float scale;
+    int* error_flag;
+    // outputs and row statistics
+    uint16_t *out0, *out1;
+    int64_t row0, head0, row1, head1;
+    float* lse;
+    const float* delta;
+};
+
+// ---------------------------------------------------------------- PTX beyond ptx_sm100.cuh
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2) {
+    asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+            "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+            : "memory");
+}
+// D (+)= A B with A in TMEM: lane = row, a 32-bit column holds two neighbours along K
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+            "{\n"
+            " .reg .pred p;\n"
+            " setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+            "}\n" ::"r"(d),
+            "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+            "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+            "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+            "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+            "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+            "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+            : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// 384 threads start with 168 registers each; the eight warps that hold rows of scores take 224, the other four
+// keep 56: 256 x 224 + 128 x 56 = 384 x 168
+__device__ __forceinline__ void registers_of_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+__device__ __forceinline__ void registers_of_others() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool FP16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (FP16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool FP16>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+    if (FP16)
+        return __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// M = 128, both operands f16 or both bf16, float32 accumulator
+template <bool FP16>
+__device__ __forceinline__ uint32_t idesc_for(int n, bool b_mn) {
+    const uint32_t f = FP16 ? 0u : 1u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(TILE >> 4) << 24);
+}
+// Tile [128 rows, dim] as an operand whose K axis is dim: step kk of 16 elements
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int kk) {
+    return umma_smem_desc_sw128(tile + (kk >> 2) * CHUNK_BYTES + (kk & 3) * 32, 16, 1024);
+}
+// The same tile as an operand whose K axis is the rows: step kk of 16 rows
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int kk) {
+    return umma_smem_desc_sw128(tile + kk * 2048, CHUNK_BYTES, 1024);
+}
+
+// ---------------------------------------------------------------- which sequence a tile belongs to
+struct Where {
+    int start, len, local;  // first row and length of the sequence, the tile's number in it; len = 0: no such tile
+    int tiles;              // tiles of the sequence
+};
+// By one whole warp.  Offsets are forced into order and range, so that no access leaves the tensors
+// whatever they hold.
+__device__ __forceinline__ Where find_tile(const Params& p, int rows, int index) {
+    Where w{0, 0, 0, 0};
+    const int lane = threadIdx.x & 31;
+    if (p.cu == nullptr) {
+        w.tiles = (p.tokens + rows - 1) / rows;
+        if (index < w.tiles)
+            w = {0, p.tokens, index, w.tiles};
+        return w;
+    }
+    for (int base = 0; base < p.seqs; base += 32) {
+        const int s = base + lane;
+        int a = 0, e = 0;
+        if (s < p.seqs) {
+            a = min(max(p.cu[s], 0), p.tokens);
+            e = min(max(p.cu[s + 1], a), p.tokens);
+        }
+        const int n = (e - a + rows - 1) / rows;
+        int upto = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o)
+                upto += v;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, upto > index);
+        if (past != 0) {
+            const int src = __ffs(past) - 1;
+            w.start = __shfl_sync(0xffffffffu, a, src);
+            w.len = __shfl_sync(0xffffffffu, e, src) - w.start;
+            w.tiles = __shfl_sync(0xffffffffu, n, src);
+            w.local = index - (__shfl_sync(0xffffffffu, upto, src) - w.tiles);
+            return w;
+        }
+        index -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return w;
+}
+
+// Loads rows [row, row + 128) of one head; `bar` counts the bytes (chunks past the dimension are not loaded)
+template <int DP>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, uint32_t bar, int head, int row) {
+    mbar_expect_tx(bar, DP / 64 * CHUNK_BYTES);
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c)
+        tma_load_3d(dst + c * CHUNK_BYTES, map, bar, c * 64, head, row);
+}
+// Zeroes rows [from, 128) of a tile (by a whole warp) for the asynchronous reads that follow
+template <int DP>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from) {
+    const int lane = threadIdx.x & 31;
+    for (int c = 0; c < DP / 64; ++c)
+        for (int i = from * 8 + lane; i < TILE * 8; i += 32)
+            reinterpret_cast<uint4*>(tile + c * CHUNK_BYTES)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+// One tile into ring slot `dst` by a whole warp.  If the sequence ends inside, the rows behind are zeroed before
+// the slot's barrier completes: the copy then arrives on `side` first.
+template <int DP>
+__device__ __forceinline__ bool feed(uint8_t* dst, const CUtensorMap* map, uint32_t full, uint32_t side, uint32_t& side_phase,
+                                     int head, int row, int live, const WaitCtx& wc) {
+    const bool cut = live < TILE;
+    if (elect_one())
+        load_tile<DP>(smem_u32(dst), map, cut ? side : full, head, row);
+    __syncwarp();
+    if (cut) {
+        const bool ok = mbar_wait(side, side_phase, wc);
+        side_phase ^= 1;
+        if (!__all_sync(0xffffffffu, ok))
+            return false;
+        zero_rows<DP>(dst, live);
+        if (elect_one())
+            mbar_arrive(full);
+        __syncwarp();
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint8_t* align_1024(uint8_t* p) {
+    return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~static_cast<uintptr_t>(1023));
+}
+
+// Writes one row of `dim` float32 TMEM columns times `f`, rounded, to global memory
+template <bool FP16>
+__device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint16_t* to, bool write) {
+    for (int c = 0; c < dim; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + c, r);
+        tmem_ld_wait(r);
+        if (!write)
+            continue;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            if (c + i < dim) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    w[k] = pack2<FP16>(__uint_as_float(r[i + 2 * k]) * f, __uint_as_float(r[i + 2 * k + 1]) * f);
+                *reinterpret_cast<uint4*>(to + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+}
+
+// ================================================================ forward
+//
+// A CTA takes two tiles of 128 queries of one head and walks over the keys once; while one warpgroup works on the
+// scores of its tile, the tensor cores work for the other tile.  The running maximum only moves when the
+// new one is more than 2^8 larger (then the accumulator is rescaled in TMEM by the threads that own its rows): P
+// stays below 2^8, which changes nothing in its relative precision, and the rescaling is rare.
+constexpr int FWD_THREADS = 384;
+constexpr int FWD_STAGES = 4;
+
+template <int DP>
+constexpr int tile_bytes() { return DP / 64 * CHUNK_BYTES; }
+template <int DP>
+constexpr int fwd_smem() { return (2 + FWD_STAGES) * tile_bytes<DP>() + 1024 + 512; }
+
+template <int DP, bool FP16>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+        forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const Params p) {
+    constexpr int TB = tile_bytes<DP>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_1024(smem_raw);
+    uint8_t* ring = smem + 2 * TB;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring + FWD_STAGES * TB);
+    const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * FWD_STAGES;
+    const uint32_t q_full = empty0 + 8 * FWD_STAGES;          // one per tile
+    const uint32_t s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 16, side = o_full + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FWD_STAGES + 9);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const int head = static_cast<int>(blockIdx.x % p.heads);
+    if (warp == 0) {
+        const Where w = find_tile(p, 2 * TILE, static_cast<int>(blockIdx.x / p.heads));
+        if (lane == 0)
+            *where = w;
+    }
+    if (warp == 9 && lane == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < 2 * FWD_STAGES; ++s)
+            mbar_init(full0 + 8 * s, 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(q_full + 8 * t, 1);
+            mbar_init(s_full + 8 * t, 1);
+            mbar_init(p_ready + 8 * t, 4);
+            mbar_init(o_full + 8 * t, 1);
+        }
+        mbar_init(side, 1);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+        prefetch_tensormap(&map_q);
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+    }
+    __syncthreads();
+    const Where w = *where;
+    if (w.len == 0)
+        return;  // all threads alike, before anything is allocated
+    if (warp == 8) {
+        tmem_alloc_cg1(smem_u32(tmem_slot), 512);
+        tmem_relinquish_cg1();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t t_s = tmem, t_o = tmem + 2 * TILE;  // S of tile t at t_s + 128 t, O at t_o + 128 t
+
+    // the last tiles of a sequence, which have the most keys, come first
+    const int r0 = (w.tiles - 1 - w.local) * 2 * TILE;
+    int n_blocks[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = r0 + t * TILE;
+        const int keys = p.causal ? min(w.len, first + TILE) : w.len;
+        n_blocks[t] = first < w.len ? (keys + TILE - 1) / TILE : 0;
+    }
+    const int n = max(n_blocks[0], n_blocks[1]);
+    WaitCtx wc{abort_flag, WAIT_NS};
+
+    if (warp == 9) {
+        registers_of_others();
+        const int kv_head = head / (p.heads / p.kv_heads);
+        if (elect_one()) {
+            load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
+            if (n_blocks[1] > 0)
+                load_tile<DP>(smem_u32(smem) + TB, &map_q, q_full + 8, head, w.start + r0 + TILE);
+        }
+        __syncwarp();
+        uint32_t side_phase = 0;
+        for (int it = 0; it < 2 * n; ++it) {
+            const int s = it % FWD_STAGES;
+            if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((it / FWD_STAGES) & 1) ^ 1, wc)))
+                break;
+            const int k0 = (it >> 1) * TILE;
+            // keys behind the end are masked where their scores are used; values are summed over
+            const int live = (it & 1) ? w.len - k0 : TILE;
+            if (!feed<DP>(ring + s * TB, (it & 1) ? &map_v : &map_k, full0 + 8 * s, side, side_phase, kv_head, w.start + k0,
+                          live, wc))
+                break;
+        }
+    } else if (warp == 8) {
+        registers_of_others();
+        if (elect_one()) {
+            const int ksteps = (p.dim + 15) / 16;
+            const uint32_t id_s = idesc_for<FP16>(TILE, false), id_o = idesc_for<FP16>(ksteps * 16, true);
+            auto scores = [&](int t, int it) {
+                const uint32_t q = smem_u32(smem) + t * TB, k = smem_u32(ring) + it % FWD_STAGES * TB;
+                for (int kk = 0; kk < ksteps; ++kk)
+                    umma_f16_cg1(t_s + t * TILE, desc_k(q, kk), desc_k(k, kk), id_s, kk != 0);
+                umma_commit_cg1(s_full + 8 * t);
+            };
+            auto loaded = [&](int it) { return mbar_wait(full0 + 8 * (it % FWD_STAGES), (it / FWD_STAGES) & 1, wc); };
+            bool ok = mbar_wait(q_full, 0, wc) && loaded(0);
+            if (ok) {
+                tc_fence_after();
+                scores(0, 0);
+                if (n_blocks[1] > 0) {
+                    ok = mbar_wait(q_full + 8, 0, wc);
+                    if (ok)
+                        scores(1, 0);
+                }
+                if (n > 2)  // the slot is used again
+                    umma_commit_cg1(empty0);
+            }
+            for (int j = 0; ok && j < n; ++j) {
+                const int iv = 2 * j + 1, ik = 2 * j + 2;
+                ok = loaded(iv);
+                const uint32_t v = smem_u32(ring) + iv % FWD_STAGES * TB;
+                bool next = false;
+                for (int t = 0; ok && t < 2; ++t) {
+                    if (j >= n_blocks[t])
+                        continue;
+                    ok = mbar_wait(p_ready + 8 * t, j & 1, wc);
+                    if (!ok)
+                        break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < TILE / 16; ++kk)
+                        umma_ts(t_o + t * TILE, t_s + t * TILE + 8 * kk, desc_mn(v, kk), id_o, j != 0 || kk != 0);
+                    if (j + 1 == n_blocks[t]) {
+                        umma_commit_cg1(o_full + 8 * t);
+                    } else {
+                        if (!next)
+                            ok = loaded(ik);
+                        next = true;
+                        if (ok) {
+                            tc_fence_after();
+                            scores(t, ik);  // over P of this block: products of one thread run in order
+                        }
+                    }
+                }
+                if (next) {  // (behind the last block nobody waits for a free slot)
+                    umma_commit_cg1(empty0 + 8 * (iv % FWD_STAGES));
+                    umma_commit_cg1(empty0 + 8 * (ik % FWD_STAGES));
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        registers_of_rows();
+        const int t = warp >> 2;
+        const int row = (threadIdx.x & 127) + r0 + t * TILE;  // in the sequence
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = t_s + t * TILE + lanes, o_at = t_o + t * TILE + lanes;
+        const float c = p.scale * LOG2E;
+        const int limit = p.causal ? min(w.len, row + 1) : w.len;  // keys that this row sees
+        float m = 0.f, l = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n_blocks[t]; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, j & 1, wc));
+            if (!ok)
+                break;
+            tc_fence_after();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                tmem_ld_32x32b_x32(s_at + 32 * i, s[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                tmem_ld_wait(s[i]);
+            const int k0 = j * TILE;
+            if (k0 + TILE > w.len || (p.causal && k0 + TILE > r0 + t * TILE)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (k0 + 32 * i + e >= limit)
+                            s[i][e] = 0xff800000u;
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    top[i] = fmaxf(top[i], __uint_as_float(s[i][e]));
+            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (j == 0) {
+                m = mx;
+            } else if (__any_sync(0xffffffffu, (mx - m) * c > 8.f)) {
+                // the product that last added to O has retired: the scores' barrier came after it
+                const float to = fmaxf(m, mx), f = ex2((m - to) * c);
+                m = to;
+                l *= f;
+                for (int d = 0; d < p.dim; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(o_at + d, o);
+                    tmem_ld_wait(o);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st_x32(o_at + d, o);
+                }
+            }
+            const float mc = m * c;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    const float a = ex2(fmaf(__uint_as_float(s[i + e / 32][e % 32]), c, -mc));
+                    const float b = ex2(fmaf(__uint_as_float(s[i + e / 32][e % 32 + 1]), c, -mc));
+                    sum[(e >> 1) & 1] += a;
+                    sum[2 + ((e >> 1) & 1)] += b;
+                    pk[e / 2] = pack2<FP16>(a, b);
+                }
+                tmem_st_x32(s_at + 16 * i, pk);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(p_ready + 8 * t);
+        }
+        if (ok && n_blocks[t] > 0 && __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, 0, wc))) {
+            tc_fence_after();
+            const bool write = row < w.len;
+            const int64_t at = w.start + row;
+            store_row<FP16>(o_at, p.dim, 1.f / l, p.out0 + at * p.row0 + head * p.head0, write);
+            if (write)
+                p.lse[static_cast<int64_t>(head) * p.tokens + at] = m * p.scale + logf(l);
+        }
+    } else {
+        registers_of_others();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8)
+        tmem_dealloc_cg1(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
+        *p.error_flag = 1;
+}
+
+// ================================================================ backward: delta
+// One warp a row and head: sums of out * dout.  Bound by reading both.
+template <bool FP16>
+__global__ void __launch_bounds__(256) delta_kernel(const uint16_t* __restrict__ out, int64_t o_row, int64_t o_head,
+                                                    const uint16_t* __restrict__ dout, int64_t d_row, int64_t d_head, int tokens,
+                                                    int heads, int dim, float* __restrict__ delta) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // half a warp a row
+    const int sub = threadIdx.x & 15;
+    const int64_t row = i / heads, head = i % heads;
+    float sum = 0.f;
+    if (row < tokens && sub * 8 < dim) {
+        const uint4 a = *reinterpret_cast<const uint4*>(out + row * o_row + head * o_head + sub * 8);
+        const uint4 b = *reinterpret_cast<const uint4*>(dout + row * d_row + head * d_head + sub * 8);
+        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float2 x = unpack2<FP16>(aw[k]), y = unpack2<FP16>(bw[k]);
+            sum += x.x * y.x + x.y * y.y;
+        }
+    }
+    for (int o = 8; o > 0; o >>= 1)
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (row < tokens && sub == 0)
+        delta[head * tokens + row] = sum;
+}
+
+// ================================================================ backward: dQ
+//
+// A CTA takes 128 queries of one head.  Both warpgroups work on every tile of scores, a thread on half a row.
+//   tensor cores:  S(j+1)         dQ += dS(j) K, dP(j+1) = dO V^T      S(j+2) ...
+//   warpgroups:    dS(j) from dP  P(j+1) from S                        dS(j+1) ...
+constexpr int BWD_THREADS = 384;  // 8 warps of arithmetic, MMA, TMA, row statistics (dK/dV only), one idle
+constexpr int BWD_STAGES = 2;
+
+template <int DP>
+constexpr int bwd_smem() { return (2 + 2 * BWD_STAGES) * tile_bytes<DP>() + BWD_STAGES * 2 * TILE * 4 + 1024 + 512; }
+
+// Half a row (64 columns) of P: TMEM column `s_at` on
+template <class F>
+__device__ __forceinline__ void half_row(uint32_t s_at, F each) {
+    uint32_t s[2][32];
+    tmem_ld_32x32b_x32(s_at, s[0]);
+    tmem_ld_32x32b_x32(s_at + 32, s[1]);
+    tmem_ld_wait(s[0]);
+    tmem_ld_wait(s[1]);
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+        each(e, __uint_as_float(s[e / 32][e % 32]));
+}
+// A operand of step kk of 16: the two halves of a row were written where their scores were
+__device__ __forceinline__ uint32_t a_half(uint32_t t, int kk) { return t + (kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)); }
+
+template <int DP, bool FP16>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+        dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
+    constexpr int TB = tile_bytes<DP>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_1024(smem_raw);  // Q, dO, then K slots, then V slots
+    uint8_t *ring_k = smem + 2 * TB, *ring_v = ring_k + BWD_STAGES * TB;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring_v + BWD_STAGES * TB + BWD_STAGES * 2 * TILE * 4);
+    const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
+    const uint32_t q_full = v_empty + 16, s_full = q_full + 8, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8,
+                   done = ds_ready + 8, side = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const int head = static_cast<int>(blockIdx.x % p.heads);
+    if (warp == 0) {
+        const Where w = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.heads));
+        if (lane == 0)
+            *where = w;
+    }
+    if (warp == 9 && lane == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < 8; ++s)
+            mbar_init(k_full + 8 * s, 1);
+        mbar_init(q_full, 2);
+        mbar_init(s_full, 1);
+        mbar_init(s_free, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_ready, 8);
+        mbar_init(done, 1);
+        mbar_init(side, 1);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    const Where w = *where;
+    if (w.len == 0)
+        return;
+    if (warp == 8) {
+        tmem_alloc_cg1(smem_u32(tmem_slot), 512);
+        tmem_relinquish_cg1();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dq = tmem + 2 * TILE;
+    const int r0 = (w.tiles - 1 - w.local) * TILE;
+    const int keys = p.causal ? min(w.len, r0 + TILE) : w.len;
+    const int n = (keys + TILE - 1) / TILE;
+    WaitCtx wc{abort_flag, WAIT_NS};
+
+    if (warp == 9) {
+        registers_of_others();
+        const int kv_head = head / (p.heads / p.kv_heads);
+        if (elect_one()) {
+            load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
+            load_tile<DP>(smem_u32(smem) + TB, &map_do, q_full, head, w.start + r0);
+        }
+        __syncwarp();
+        uint32_t side_phase = 0;
+        for (int j = 0; j < n; ++j) {
+            const int s = j % BWD_STAGES, live = w.len - j * TILE;
+            const uint32_t ph = ((j / BWD_STAGES) & 1) ^ 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * s, ph, wc)) ||
+                !feed<DP>(ring_k + s * TB, &map_k, k_full + 8 * s, side, side_phase, kv_head, w.start + j * TILE, live, wc))
+                break;
+            if (!__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * s, ph, wc)) ||
+                !feed<DP>(ring_v + s * TB, &map_v, v_full + 8 * s, side, side_phase, kv_head, w.start + j * TILE, live, wc))
+                break;
+        }
+    } else if (warp == 8) {
+        registers_of_others();
+        if (elect_one()) {
+            const int ksteps = (p.dim + 15) / 16;
+            const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
+            const uint32_t q = smem_u32(smem), d_o = q + TB;
+            auto scores = [&](int j) {
+                const int s = j % BWD_STAGES;
+                if (!mbar_wait(k_full + 8 * s, (j / BWD_STAGES) & 1, wc))
+                    return false;
+                tc_fence_after();
+                for (int kk = 0; kk < ksteps; ++kk)
+                    umma_f16_cg1(t_s, desc_k(q, kk), desc_k(smem_u32(ring_k) + s * TB, kk), id_s, kk != 0);
+                umma_commit_cg1(s_full);
+                return true;
+            };
+            auto grads = [&](int j) {
+                const int s = j % BWD_STAGES;
+                if (!mbar_wait(v_full + 8 * s, (j / BWD_STAGES) & 1, wc))
+                    return false;
+                tc_fence_after();
+                for (int kk = 0; kk < ksteps; ++kk)
+                    umma_f16_cg1(t_dp, desc_k(d_o, kk), desc_k(smem_u32(ring_v) + s * TB, kk), id_s, kk != 0);
+                umma_commit_cg1(dp_full);
+                umma_commit_cg1(v_empty + 8 * s);
+                return true;
+            };
+            bool ok = mbar_wait(q_full, 0, wc) && scores(0) && grads(0);
+            for (int j = 0; ok && j < n; ++j) {
+                if (j + 1 < n)
+                    ok = mbar_wait(s_free, j & 1, wc) && scores(j + 1);
+                ok = ok && mbar_wait(ds_ready, j & 1, wc);
+                if (!ok)
+                    break;
+                tc_fence_after();
+                const uint32_t k = smem_u32(ring_k) + j % BWD_STAGES * TB;
+#pragma unroll
+                for (int kk = 0; kk < TILE / 16; ++kk)
+                    umma_ts(t_dq, a_half(t_dp, kk), desc_mn(k, kk), id_d, j != 0 || kk != 0);
+                umma_commit_cg1(k_empty + 8 * (j % BWD_STAGES));
+                if (j + 1 < n)
+                    ok = grads(j + 1);
+            }
+            if (ok)
+                umma_commit_cg1(done);
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        registers_of_rows();
+        const int half = warp >> 2;
+        const int row = (threadIdx.x & 127) + r0;
+        const bool live = row < w.len;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const float c = p.scale * LOG2E;
+        const int limit = p.causal ? min(w.len, row + 1) : w.len;
+        const int64_t at = static_cast<int64_t>(head) * p.tokens + w.start + row;
+        const float lse2 = live ? p.lse[at] * LOG2E : 0.f, delta = live ? p.delta[at] : 0.f;
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int k0 = j * TILE + half * 64;
+            float pr[64];
+            ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, wc));
+            if (!ok)
+                break;
+            tc_fence_after();
+            half_row(t_s + half * 64 + lanes, [&](int e, float s) { pr[e] = s; });
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(s_free);
+#pragma unroll
+            for (int e = 0; e < 64; ++e)
+                pr[e] = ex2(fmaf(pr[e], c, -lse2));
+            if (j * TILE + TILE > w.len || (p.causal && j * TILE + TILE > r0)) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                    if (k0 + e >= limit)
+                        pr[e] = 0.f;
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(dp_full, j & 1, wc));
+            if (!ok)
+                break;
+            tc_fence_after();
+            uint32_t pk[32];
+            half_row(t_dp + half * 64 + lanes, [&](int e, float dp) {
+                pr[e] *= dp - delta;
+                if (e & 1)
+                    pk[e / 2] = pack2<FP16>(pr[e - 1], pr[e]);
+            });
+            tmem_st_x32(t_dp + half * 64 + lanes, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(ds_ready);
+        }
+        if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, wc))) {
+            tc_fence_after();
+            if (half == 0)
+                store_row<FP16>(t_dq + lanes, p.dim, p.scale, p.out0 + (w.start + static_cast<int64_t>(row)) * p.row0 + head * p.head0, live);
+        }
+    } else {
+        registers_of_others();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8)
+        tmem_dealloc_cg1(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
+        *p.error_flag = 1;
+}
+
+// ================================================================ backward: dK and dV
+//
+// A CTA takes 128 keys of one key / value head and walks over the queries of every head of its group; rows of the
+// score tiles are keys, so P^T and dS^T are left operands as they stand.
+//   tensor cores:  dV += P^T(i) dO, S^T(i+1)    dK += dS^T(i) Q, dP^T(i+1)
+//   warpgroups:    dS(i) from dP                P(i+1) from S
+template <int DP, bool FP16>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+        dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
+    constexpr int TB = tile_bytes<DP>();
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = align_1024(smem_raw);  // K, V, then Q slots, then dO slots, then lse and delta of the slots' rows
+    uint8_t *ring_q = smem + 2 * TB, *ring_do = ring_q + BWD_STAGES * TB;
+    float* stats = reinterpret_cast<float*>(ring_do + BWD_STAGES * TB);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stats + BWD_STAGES * 2 * TILE);
+    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 16, o_full = q_empty + 16, o_empty = o_full + 16;
+    const uint32_t st_full = o_empty + 16, st_empty = st_full + 16;
+    const uint32_t kv_full = st_empty + 16, s_full = kv_full + 8, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
+                   done = ds_ready + 8, side = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const int lane = threadIdx.x & 31;
+    const int kv_head = static_cast<int>(blockIdx.x % p.kv_heads);
+    const int group = p.heads / p.kv_heads;
+    if (warp == 0) {
+        const Where w = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.kv_heads));
+        if (lane == 0)
+            *where = w;
+    }
+    if (warp == 9 && lane == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < 8; ++s)
+            mbar_init(q_full + 8 * s, 1);
+        for (int s = 0; s < BWD_STAGES; ++s) {
+            mbar_init(st_full + 8 * s, 1);
+            mbar_init(st_empty + 8 * s, 8);
+        }
+        mbar_init(kv_full, 2);
+        mbar_init(s_full, 1);
+        mbar_init(p_ready, 8);
+        mbar_init(dp_full, 1);
+        mbar_init(ds_ready, 8);
+        mbar_init(done, 1);
+        mbar_init(side, 1);
+        mbar_fence_init();
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    const Where w = *where;
+    if (w.len == 0)
+        return;
+    if (warp == 8) {
+        tmem_alloc_cg1(smem_u32(tmem_slot), 512);
+        tmem_relinquish_cg1();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 3 * TILE;
+    const int k0 = w.local * TILE;               // the first keys, which the most queries see, come first
+    const int i0 = p.causal ? w.local : 0;       // first block of queries that sees them
+    const int per_head = w.tiles - i0;
+    const int n = group * per_head;
+    WaitCtx wc{abort_flag, WAIT_NS};
+
+    if (warp == 9) {
+        registers_of_others();
+        if (elect_one()) {
+            load_tile<DP>(smem_u32(smem), &map_k, kv_full, kv_head, w.start + k0);
+            load_tile<DP>(smem_u32(smem) + TB, &map_v, kv_full, kv_head, w.start + k0);
+        }
+        __syncwarp();
+        uint32_t side_phase = 0;
+        for (int it = 0; it < n; ++it) {
+            const int s = it % BWD_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
+            const uint32_t ph = ((it / BWD_STAGES) & 1) ^ 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(q_empty + 8 * s, ph, wc)) ||
+                !feed<DP>(ring_q + s * TB, &map_q, q_full + 8 * s, side, side_phase, head, w.start + q0, w.len - q0, wc))
+                break;
+            if (!__all_sync(0xffffffffu, mbar_wait(o_empty + 8 * s, ph, wc)) ||
+                !feed<DP>(ring_do + s * TB, &map_do, o_full + 8 * s, side, side_phase, head, w.start + q0, w.len - q0, wc))
+                break;
+        }
+    } else if (warp == 10) {
+        registers_of_others();
+        // lse (times log2 e) and delta of every block's rows; a row behind the end has probabilities of zero
+        for (int it = 0; it < n; ++it) {
+            const int s = it % BWD_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
+            if (!__all_sync(0xffffffffu, mbar_wait(st_empty + 8 * s, ((it / BWD_STAGES) & 1) ^ 1, wc)))
+                break;
+            float* to = stats + s * 2 * TILE;
+            const int64_t at = static_cast<int64_t>(head) * p.tokens + w.start + q0;
+            for (int r = lane; r < TILE; r += 32) {
+                const bool live = q0 + r < w.len;
+                to[r] = live ? p.lse[at + r] * LOG2E : INFINITY;
+                to[TILE + r] = live ? p.delta[at + r] : 0.f;
+            }
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(st_full + 8 * s);
+        }
+    } else if (warp == 8) {
+        registers_of_others();
+        if (elect_one()) {
+            const int ksteps = (p.dim + 15) / 16;
+            const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
+            const uint32_t k = smem_u32(smem), v = k + TB;
+            auto scores = [&](int it) {
+                const int s = it % BWD_STAGES;
+                if (!mbar_wait(q_full + 8 * s, (it / BWD_STAGES) & 1, wc))
+                    return false;
+                tc_fence_after();
+                for (int kk = 0; kk < ksteps; ++kk)
+                    umma_f16_cg1(t_s, desc_k(k, kk), desc_k(smem_u32(ring_q) + s * TB, kk), id_s, kk != 0);
+                umma_commit_cg1(s_full);
+                return true;
+            };
+            auto grads = [&](int it) {
+                const int s = it % BWD_STAGES;
+                if (!mbar_wait(o_full + 8 * s, (it / BWD_STAGES) & 1, wc))
+                    return false;
+                tc_fence_after();
+                for (int kk = 0; kk < ksteps; ++kk)
+                    umma_f16_cg1(t_dp, desc_k(v, kk), desc_k(smem_u32(ring_do) + s * TB, kk), id_s, kk != 0);
+                umma_commit_cg1(dp_full);
+                return true;
+            };
+            bool ok = mbar_wait(kv_full, 0, wc) && scores(0) && grads(0);
+            for (int it = 0; ok && it < n; ++it) {
+                const int s = it % BWD_STAGES;
+                ok = mbar_wait(p_ready, it & 1, wc);
+                if (!ok)
+                    break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < TILE / 16; ++kk)
+                    umma_ts(t_dv, a_half(t_s, kk), desc_mn(smem_u32(ring_do) + s * TB, kk), id_d, it != 0 || kk != 0);
+                umma_commit_cg1(o_empty + 8 * s);
+                if (it + 1 < n)
+                    ok = scores(it + 1);
+                ok = ok && mbar_wait(ds_ready, it & 1, wc);
+                if (!ok)
+                    break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < TILE / 16; ++kk)
+                    umma_ts(t_dk, a_half(t_dp, kk), desc_mn(smem_u32(ring_q) + s * TB, kk), id_d, it != 0 || kk != 0);
+                umma_commit_cg1(q_empty + 8 * s);
+                if (it + 1 < n)
+                    ok = grads(it + 1);
+            }
+            if (ok)
+                umma_commit_cg1(done);
+        }
+        __syncwarp();
+    } else if (warp < 8) {
+        registers_of_rows();
+        const int half = warp >> 2;
+        const int key = (threadIdx.x & 127) + k0;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const float c = p.scale * LOG2E;
+        bool ok = true;
+        for (int it = 0; it < n; ++it) {
+            const int s = it % BWD_STAGES, q0 = (i0 + it % per_head) * TILE + half * 64;
+            const float4* lse2 = reinterpret_cast<const float4*>(stats + s * 2 * TILE + half * 64);
+            const float4* delta = lse2 + TILE / 4;
+            float pr[64];
+            ok = __all_sync(0xffffffffu, mbar_wait(st_full + 8 * s, (it / BWD_STAGES) & 1, wc) && mbar_wait(s_full, it & 1, wc));
+            if (!ok)
+                break;
+            tc_fence_after();
+            half_row(t_s + half * 64 + lanes, [&](int e, float x) { pr[e] = x; });
+#pragma unroll
+            for (int e = 0; e < 64; e += 4) {
+                const float4 z = lse2[e / 4];
+                pr[e] = ex2(fmaf(pr[e], c, -z.x));
+                pr[e + 1] = ex2(fmaf(pr[e + 1], c, -z.y));
+                pr[e + 2] = ex2(fmaf(pr[e + 2], c, -z.z));
+                pr[e + 3] = ex2(fmaf(pr[e + 3], c, -z.w));
+            }
+            if (p.causal && it % per_head == 0) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e)
+                    if (q0 + e < key)
+                        pr[e] = 0.f;
+            }
+            uint32_t pk[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                pk[e] = pack2<FP16>(pr[2 * e], pr[2 * e + 1]);
+            tmem_st_x32(t_s + half * 64 + lanes, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(p_ready);
+            ok = __all_sync(0xffffffffu, mbar_wait(dp_full, it & 1, wc));
+            if (!ok)
+                break;
+            tc_fence_after();
+            half_row(t_dp + half * 64 + lanes, [&](int e, float dp) {
+                const float4 d = delta[e / 4];
+                pr[e] *= dp - (e % 4 == 0 ? d.x : e % 4 == 1 ? d.y : e % 4 == 2 ? d.z : d.w);
+                if (e & 1)
+                    pk[e / 2] = pack2<FP16>(pr[e - 1], pr[e]);
+            });
+            tmem_st_x32(t_dp + half * 64 + lanes, pk);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(st_empty + 8 * s);
+                mbar_arrive(ds_ready);
+            }
+        }
+        if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, wc))) {
+            tc_fence_after();
+            const bool live = key < w.len;
+            const int64_t at = w.start + static_cast<int64_t>(key);
+            if (half == 0)
+                store_row<FP16>(t_dk + lanes, p.dim, p.scale, p.out0 + at * p.row0 + kv_head * p.head0, live);
+            else
+                store_row<FP16>(t_dv + lanes, p.dim, 1.f, p.out1 + at * p.row1 + kv_head * p.head1, live);
+        }
+    } else {
+        registers_of_others();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8)
+        tmem_dealloc_cg1(tmem, 512);
+    if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
+        *p.error_flag = 1;
+}
+
+// ================================================================ host side
+// [tokens, heads, dim] with boxes of 128 rows x 1 head x 64 elements; columns past the dimension and rows
+// past the tensor read as zero
+bool make_map(CUtensorMap* map, const Tensor& t, int heads, const Problem& p) {
+    auto fn = mgk::gemm::get_encode_fn();
+    if (fn == nullptr)
+        return false;
+    cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(p.tokens)};
+    cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.head) * 2, static_cast<cuuint64_t>(t.row) * 2};
+    cuuint32_t box[3] = {64, 1, TILE};
+    cuuint32_t step[3] = {1, 1, 1};
+    return fn(map, p.fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, t.p, dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool bad(const Tensor& t) {
+    constexpr int64_t most = int64_t{1} << 38;  // strides of a tensor map are below 2^40 bytes
+    return t.p == nullptr || (reinterpret_cast<uintptr_t>(t.p) & 15) || t.row <= 0 || t.head <= 0 || t.row % 8 || t.head % 8 ||
+           t.row >= most || t.head >= most;
+}
+bool bad(const Problem& p) {
+    return p.tokens < 0 || p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads || p.dim < 8 || p.dim > kMaxDim || p.dim % 8 ||
+           p.seqs < 0 || (p.cu != nullptr && p.seqs < 1) || (reinterpret_cast<uintptr_t>(p.cu) & 3) || !(p.scale > 0.f) ||
+           !(p.scale < INFINITY);
+}
+// CTAs that cover every possible cut of the rows into sequences, `rows` of one sequence and `heads` heads each;
+// 0 when there are too many
+unsigned grid_for(const Problem& p, int rows, int heads) {
+    const int64_t seqs = p.cu != nullptr ? p.seqs : 1;
+    const int64_t tiles = (p.tokens + seqs * (rows - 1)) / rows;
+    const int64_t most = p.tokens < tiles ? p.tokens : tiles;
+    const int64_t ctas = (p.cu != nullptr ? most : (p.tokens + rows - 1) / rows) * heads;
+    return ctas > 0x7fffffff ? 0u : static_cast<unsigned>(ctas);
+}
+Params params(const Problem& p) {
+    Params k{};
+    k.cu = p.cu;
+    k.seqs = p.seqs;
+    k.tokens = p.tokens;
+    k.heads = p.heads;
+    k.kv_heads = p.kv_heads;
+    k.dim = p.dim;
+    k.causal = p.causal;
+    k.scale = p.scale;
+    k.error_flag = p.error_flag;
+    return k;
+}
+template <class F>
+cudaError_t pick(const Problem& p, F go) {
+    using T = std::true_type;
+    using N = std::false_type;
+    if (p.dim <= 64)
+        return p.fp16 ? go(std::integral_constant<int, 64>{}, T{}) : go(std::integral_constant<int, 64>{}, N{});
+    return p.fp16 ? go(std::integral_constant<int, 128>{}, T{}) : go(std::integral_constant<int, 128>{}, N{});
+}
+// (the attribute belongs to a function on a device: it is set before every launch, which costs under a microsecond)
+template <class K, class... A>
+cudaError_t run(K kernel, unsigned grid, int threads, int smem, cudaStream_t stream, A... args) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess)
+        return e;
+    kernel<<<grid, threads, smem, stream>>>(args...);
+    count_launch();
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tensor out, float* lse, cudaStream_t stream) {
+    if (bad(p))
+        return cudaErrorInvalidValue;
+    if (p.tokens == 0)
+        return cudaSuccess;
+    if (bad(q) || bad(k) || bad(v) || bad(out) || lse == nullptr || (reinterpret_cast<uintptr_t>(lse) & 3))
+        return cudaErrorInvalidValue;
+    const unsigned grid = grid_for(p, 2 * TILE, p.heads);
+    CUtensorMap mq, mk, mv;
+    if (grid == 0 || !make_map(&mq, q, p.heads, p) || !make_map(&mk, k, p.kv_heads, p) || !make_map(&mv, v, p.kv_heads, p))
+        return cudaErrorInvalidValue;
+    Params a = params(p);
+    a.out0 = static_cast<uint16_t*>(out.p);
+    a.row0 = out.row;
+    a.head0 = out.head;
+    a.lse = lse;
+    return pick(p, [&](auto dp, auto half) {
+        constexpr int DP = decltype(dp)::value;
+        return run(forward_kernel<DP, decltype(half)::value>, grid, FWD_THREADS, fwd_smem<DP>(), stream, mq, mk, mv, a);
+    });
+}
+
+cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, const float* lse,
+                            Tensor dq, Tensor dk, Tensor dv, float* delta, cudaStream_t stream) {
+    if (bad(p))
+        return cudaErrorInvalidValue;
+    if (p.tokens == 0)
+        return cudaSuccess;
+    if (bad(dout) || bad(q) || bad(k) || bad(v) || bad(out) || bad(dq) || bad(dk) || bad(dv) || lse == nullptr || delta == nullptr ||
+        ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(delta)) & 3))
+        return cudaErrorInvalidValue;
+    const unsigned grid_q = grid_for(p, TILE, p.heads), grid_k = grid_for(p, TILE, p.kv_heads);
+    const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
+    CUtensorMap mq, mk, mv, mo;
+    if (grid_q == 0 || grid_k == 0 || (rows + 15) / 16 > 0x7fffffff || !make_map(&mq, q, p.heads, p) ||
+        !make_map(&mk, k, p.kv_heads, p) || !make_map(&mv, v, p.kv_heads, p) || !make_map(&mo, dout, p.heads, p))
+        return cudaErrorInvalidValue;
+    auto delta_go = [&](auto kernel) {
+        kernel<<<static_cast<unsigned>((rows + 15) / 16), 256, 0, stream>>>(
+                static_cast<const uint16_t*>(out.p), out.row, out.head, static_cast<const uint16_t*>(dout.p), dout.row, dout.head,
+                p.tokens, p.heads, p.dim, delta);
+    };
+    p.fp16 ? delta_go(delta_kernel<true>) : delta_go(delta_kernel<false>);
+    count_launch();
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess)
+        return e;
+    Params a = params(p);
+    a.lse = const_cast<float*>(lse);
+    a.delta = delta;
+    return pick(p, [&](auto dp, auto half) {
+        constexpr int DP = decltype(dp)::value;
+        constexpr bool FP16 = decltype(half)::value;
+        a.out0 = static_cast<uint16_t*>(dk.p);
+        a.row0 = dk.row;
+        a.head0 = dk.head;
+        a.out1 = static_cast<uint16_t*>(dv.p);
+        a.row1 = dv.row;
+        a.head1 = dv.head;
+        const cudaError_t first = run(dkv_kernel<DP, FP16>, grid_k, BWD_THREADS, bwd_smem<DP>(), stream, mq, mk, mv, mo, a);
+        if (first != cudaSuccess)
+            return first;
+        a.out0 = static_cast<uint16_t*>(dq.p);
+        a.row0 = dq.row;
+        a.head0 = dq.head;
+        return run(dq_kernel<DP, FP16>, grid_q, BWD_THREADS, bwd_smem<DP>(), stream, mq, mk, mv, mo, a);
+    });
+}
+
+}  // namespace attn
+}  // namespace mgk

@@ -1,0 +1,354 @@
+"""Packed attention and its backward pass against float64: lengths around the tiles, one token, empty sequences,
+grouped heads, odd head sizes, strided operands, rows behind the last sequence, refusals."""
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+HALF = {BF: 2.0 ** -8, HF: 2.0 ** -11}  # half a step, relative
+
+
+def ends(lengths):
+    return torch.tensor([0] + list(lengths)).cumsum(0).to(torch.int32).cuda()
+
+
+def make(lengths, heads, kv_heads, dim, dtype, tail=0, seed=0, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rows = sum(lengths) + tail
+    r = lambda h: (torch.randn(rows, h, dim, generator=g, device="cuda") * scale).to(dtype)  # noqa: E731
+    return r(heads), r(kv_heads), r(kv_heads), r(heads)
+
+
+def reference(q, k, v, do, lengths, causal, scale=None):
+    """out, lse, dq, dk, dv in float64 with, for each, the sum of absolute values of what was added up (the size to
+    which a rounded probability or score gradient counts)."""
+    scale = 1.0 / math.sqrt(q.shape[2]) if scale is None else scale
+    h, hk = q.shape[1], k.shape[1]
+    val = {n: torch.zeros_like(t, dtype=torch.float64) for n, t in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
+    size = {n: torch.zeros_like(t) for n, t in val.items()}
+    lse = torch.full((h, q.shape[0]), math.nan, dtype=torch.float64, device=q.device)
+    b = 0
+    for n in lengths:
+        s, b = slice(b, b + n), b + n
+        for i in range(h):
+            j = i * hk // h
+            Q, K, V, D = (t[s, x].double() for t, x in ((q, i), (k, j), (v, j), (do, i)))
+            z = Q @ K.t() * scale
+            if causal:
+                z = z.masked_fill(torch.ones_like(z, dtype=torch.bool).triu(1), -math.inf)
+            p = torch.softmax(z, 1)
+            val["out"][s, i], size["out"][s, i] = p @ V, p @ V.abs()
+            lse[i, s] = torch.logsumexp(z, 1)
+            dp = D @ V.t()
+            delta = (D * val["out"][s, i]).sum(1, keepdim=True)
+            ds = p * (dp - delta)
+            val["dv"][s, j] += p.t() @ D
+            size["dv"][s, j] += p.t() @ D.abs()
+            val["dq"][s, i] = scale * ds @ K
+            val["dk"][s, j] += scale * ds.t() @ Q
+            # delta is formed from the rounded output: off by half a step of every term
+            da = p * (dp.abs() + delta.abs() + (D.abs() * size["out"][s, i]).sum(1, keepdim=True))
+            size["dq"][s, i] = scale * da @ K.abs()
+            size["dk"][s, j] += scale * da.t() @ Q.abs()
+    return val, size, lse
+
+
+# A probability (or score gradient) is rounded once to the operands' type, by half a step of itself; its exponent's
+# argument is off by a few float32 steps of a score, 2^-13 in all here; the result is rounded once more.
+def check(got, want, size, dtype, name):
+    tol = want.abs() * HALF[dtype] + size * (HALF[dtype] + 2.0 ** -13) * 1.01 + (2.0 ** -24 if dtype == HF else 0.0)
+    off = (got.double() - want).abs()
+    assert bool((off <= tol).all()), (name, float((off / tol).nan_to_num(0.0, 9e9, 9e9).max()))
+
+
+def run_and_check(lengths, heads, kv_heads, dim, dtype, causal, tail=0, backward=True, scale=None, seed=0):
+    from megray_b200.ops import attention, attention_bwd, gemm_error_flag
+
+    q, k, v, do = make(lengths, heads, kv_heads, dim, dtype, tail, seed)
+    n = sum(lengths)
+    for t in (q, k, v, do):
+        t[n:] = float("nan")  # what lies behind the last sequence reaches nothing
+    cu = ends(lengths)
+    out = torch.full_like(q, 7.0)
+    lse = torch.full((heads, n + tail), 7.0, device="cuda")
+    attention(q, k, v, cu, causal=causal, scale=scale, out=out, lse=lse)
+    val, size, lse_want = reference(q, k, v, do, lengths, causal, scale)
+    torch.cuda.synchronize()
+    assert int(gemm_error_flag().item()) == 0
+    check(out[:n], val["out"][:n], size["out"][:n], dtype, "out")
+    # scores are sums of up to 128 products, the exponent's argument a few steps off
+    assert bool(((lse[:, :n].double() - lse_want[:, :n]).abs() <= 2.0 ** -14).all())
+    assert bool((out[n:] == 7.0).all()) and bool((lse[:, n:] == 7.0).all())
+    if not backward:
+        return
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    attention_bwd(do, q, k, v, out, lse, cu, causal=causal, scale=scale, dq=grads[0], dk=grads[1], dv=grads[2])
+    torch.cuda.synchronize()
+    assert int(gemm_error_flag().item()) == 0
+    for g, name in zip(grads, ("dq", "dk", "dv")):
+        check(g[:n], val[name][:n], size[name][:n], dtype, name)
+        assert bool((g[n:] == 7.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths", [[1], [2], [16], [127], [128], [129], [255], [256], [257], [384], [700]])
+def test_one_sequence(lengths, causal):
+    run_and_check(lengths, 2, 1, 64, BF, causal)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dim", [8, 16, 24, 40, 64, 72, 80, 96, 112, 120, 128])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_head_sizes(dim, dtype, causal):
+    run_and_check([130, 1, 61], 2, 2, dim, dtype, causal, tail=3, seed=dim)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (3, 1), (4, 2), (6, 3), (7, 1), (8, 8), (12, 4), (16, 1)])
+def test_grouped_heads(heads, kv_heads, causal):
+    run_and_check([300, 77], heads, kv_heads, 64, BF, causal, tail=1)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,tail", [([0, 5, 0, 0, 130, 1, 0], 9), ([1] * 40, 0), ([3, 129, 260, 128, 17], 200),
+                                          (list(range(1, 70)), 0), ([1000, 1, 513], 64)])
+def test_many_sequences(lengths, tail, causal):
+    run_and_check(lengths, 2, 1, 128, BF, causal, tail=tail)
+
+
+@gpu
+@pytest.mark.parametrize("causal,dtype,dim", [(True, BF, 128), (False, HF, 128), (True, HF, 64), (False, BF, 80)])
+def test_long_sequences(causal, dtype, dim):
+    run_and_check([2500, 1111], 4, 2, dim, dtype, causal, seed=5)
+
+
+@gpu
+@pytest.mark.parametrize("scale", [2.0 ** -20, 0.5, 3.0])
+def test_scales(scale):
+    from megray_b200.ops import attention
+
+    # a large scale makes the maximum jump from block to block, which rescales the accumulator
+    lengths = [600, 200]
+    q, k, v, do = make(lengths, 2, 1, 64, BF, seed=3)
+    k *= torch.linspace(0.1, 1.5, sum(lengths), device="cuda").to(BF)[:, None, None]
+    out, lse = attention(q, k, v, ends(lengths), causal=True, scale=scale)
+    val, size, lse_want = reference(q, k, v, do, lengths, True, scale)
+    # scores of up to 40 x scale, each off by 2^-20 of the sum of absolute products
+    off = (q.double().abs().amax() * k.double().abs().amax() * 64 * scale * 2.0 ** -22)
+    tol = val["out"].abs() * HALF[BF] + size["out"] * (HALF[BF] + 2 * float(off) + 2.0 ** -13)
+    assert bool(((out.double() - val["out"]).abs() <= tol).all())
+    assert bool(((lse.double() - lse_want).abs() <= 2.0 ** -14 + 2 * float(off)).all())
+
+
+@gpu
+def test_a_peak_in_every_block():
+    """One key per block of 128 outweighs everything before it: the maximum moves in every block."""
+    from megray_b200.ops import attention
+
+    n = 1024
+    q = torch.ones(n, 1, 64, device="cuda", dtype=BF)
+    k = torch.zeros(n, 1, 64, device="cuda", dtype=BF)
+    for b in range(8):
+        k[b * 128 + 60] = 1.0 + 4 * b
+    v = torch.randn(n, 1, 64, device="cuda").to(BF)
+    out, lse = attention(q, k, v, causal=True)
+    val, size, lse_want = reference(q, k, v, q, [n], True)
+    check(out, val["out"], size["out"], BF, "out")
+    assert bool(((lse.double() - lse_want).abs() <= 2.0 ** -12).all())  # scores up to 232: half steps of 2^-17
+
+
+@gpu
+def test_strided_operands():
+    from megray_b200.ops import attention, attention_bwd
+
+    rows, h, hk, d = 333, 4, 2, 72
+    qkv = torch.randn(rows, h + 2 * hk, d, device="cuda").to(BF)
+    parts = qkv[:, :h], qkv[:, h:h + hk], qkv[:, h + hk:]
+    plain = [t.contiguous() for t in parts]
+    do = torch.randn(h, rows, d, device="cuda").to(BF).transpose(0, 1)  # heads outermost
+    cu = ends([200, 133])
+    out, lse = attention(*parts, cu)
+    out2, lse2 = attention(*plain, cu)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    grad = torch.zeros(rows, h + 2 * hk, d, device="cuda", dtype=BF)
+    views = grad[:, :h], grad[:, h:h + hk], grad[:, h + hk:]
+    attention_bwd(do, *parts, out, lse, cu, dq=views[0], dk=views[1], dv=views[2])
+    for a, b in zip(views, attention_bwd(do.contiguous(), *plain, out2, lse2, cu)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_other_sequences_do_not_matter():
+    from megray_b200.ops import attention, attention_bwd
+
+    lengths = [100, 200, 50]
+    q, k, v, do = make(lengths, 2, 1, 64, BF)
+    s = slice(100, 300)
+    alone = attention(q[s], k[s], v[s])
+    alone_bwd = attention_bwd(do[s], q[s], k[s], v[s], *alone)
+    for t in (q, k, v, do):
+        t[:100] = float("nan")
+        t[300:] = float("inf")
+    out, lse = attention(q, k, v, ends(lengths))
+    grads = attention_bwd(do, q, k, v, out, lse, ends(lengths))
+    assert torch.equal(out[s], alone[0]) and torch.equal(lse[:, s], alone[1])
+    for a, b in zip(grads, alone_bwd):
+        assert torch.equal(a[s], b)
+
+
+@gpu
+def test_gradients_against_differences():
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = (t.to(HF) for t in make([70, 9], 2, 1, 32, HF, seed=8))
+    cu = ends([70, 9])
+    out, lse = attention(q, k, v, cu)
+    grads = attention_bwd(do, q, k, v, out, lse, cu)
+    # along a direction, by the definition in float64 (the kernel's own output is too coarse to difference)
+    for x, g in zip((0, 1, 2), grads):
+        way = torch.randn(g.shape, device="cuda", dtype=torch.float64)
+        loss = []
+        for s in (1, -1):
+            a = [q.double(), k.double(), v.double()]
+            a[x] = a[x] + s * 2.0 ** -10 * way
+            val, _, _ = reference(*a, do, [70, 9], True)
+            loss.append(float((val["out"] * do.double()).sum()))
+        slope = (loss[0] - loss[1]) / 2.0 ** -9
+        got = float((g.double() * way).sum())
+        # every gradient is off by at most 2^-9 of terms whose sum is below |g|_1 + 64
+        assert abs(got - slope) <= 2.0 ** -9 * (float((g.double().abs() * way.abs()).sum()) + 64)
+
+
+@gpu
+def test_the_same_bits_every_time_and_from_a_graph():
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([500, 300], 4, 2, 128, BF)
+    cu = ends([500, 300])
+    first = [*attention(q, k, v, cu)]
+    first += attention_bwd(do, q, k, v, *first, cu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [*attention(q, k, v, cu)]
+        got += attention_bwd(do, q, k, v, *got, cu)
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    # a graph follows the offsets: they are read on the device
+    cu.copy_(ends([300, 500]))
+    graph.replay()
+    again = [*attention(q, k, v, cu)]
+    assert torch.equal(got[0], again[0]) and not torch.equal(got[0], first[0])
+
+
+@gpu
+def test_two_streams_at_once():
+    from megray_b200.ops import attention, attention_bwd
+
+    sets = [make([400, 150], 4, 2, 64, BF, seed=s) for s in (1, 2)]
+    cu = ends([400, 150])
+    want = [[*attention(q, k, v, cu)] for q, k, v, _ in sets]
+    want = [w + [*attention_bwd(do, q, k, v, *w, cu)] for w, (q, k, v, do) in zip(want, sets)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for stream, (q, k, v, do) in zip(streams, sets):
+        with torch.cuda.stream(stream):
+            o = [*attention(q, k, v, cu)]
+            got.append(o + [*attention_bwd(do, q, k, v, *o, cu)])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+def test_offsets_out_of_range_touch_nothing_outside():
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([256], 1, 1, 64, BF)
+    for bad in ([-5, 100, 9000], [200, 100, 50], [0, 2 ** 31 - 1, -2 ** 31], [300, 400, 500]):
+        cu = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        out, lse = attention(q, k, v, cu)
+        attention_bwd(do, q, k, v, torch.zeros_like(out), torch.zeros_like(lse), cu)
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_no_rows():
+    from megray_b200.ops import attention, attention_bwd
+
+    q = torch.zeros(0, 2, 64, device="cuda", dtype=BF)
+    out, lse = attention(q, q, q)
+    assert out.shape == (0, 2, 64) and lse.shape == (2, 0)
+    assert all(g.shape == (0, 2, 64) for g in attention_bwd(q, q, q, q, out, lse))
+    q = torch.zeros(5, 2, 64, device="cuda", dtype=BF)
+    attention(q, q, q, torch.zeros(4, dtype=torch.int32, device="cuda"))  # only empty sequences
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_refusals():
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([64], 4, 2, 64, BF)
+    cu = ends([64])
+    wide = torch.zeros(64, 4, 68, device="cuda", dtype=BF)
+    for bad in (dict(q=q.float()), dict(q=q[0]), dict(k=k.half()), dict(k=k[:5]), dict(v=v[:, :1]), dict(k=k[:, :0], v=v[:, :0]),
+                dict(k=q[:, :3], v=q[:, :3]), dict(q=wide[..., :60], k=wide[:, :2, :60], v=wide[:, :2, :60]),
+                dict(q=wide[..., 4:68]), dict(q=q.transpose(1, 2).contiguous().transpose(1, 2)), dict(cu_seqlens=cu.long()),
+                dict(cu_seqlens=cu[:1]), dict(cu_seqlens=cu.cpu()), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                dict(scale=math.inf), dict(out=q[:5]), dict(out=q[:, :1].expand(64, 4, 64)), dict(lse=torch.zeros(4, 63, device="cuda")),
+                dict(lse=torch.zeros(64, 4, device="cuda").t()), dict(q=q.cpu())):
+        kw = {"q": q, "k": k, "v": v, "cu_seqlens": cu, **bad}
+        with pytest.raises(ValueError):
+            attention(kw.pop("q"), kw.pop("k"), kw.pop("v"), kw.pop("cu_seqlens"), **kw)
+    big = torch.zeros(8, 1, 136, device="cuda", dtype=BF)
+    with pytest.raises(ValueError):
+        attention(big, big, big)
+    out, lse = attention(q, k, v, cu)
+    for bad in (dict(dout=do[:5]), dict(dout=do.half()), dict(out=None), dict(lse=None), dict(lse=lse[:2]), dict(dk=q), dict(dq=k)):
+        kw = {"dout": do, "out": out, "lse": lse, **bad}
+        with pytest.raises(ValueError):
+            attention_bwd(kw.pop("dout"), q, k, v, kw.pop("out"), kw.pop("lse"), cu, **kw)
+
+
+def test_cpu_tensors_are_refused():
+    from megray_b200.ops import attention, attention_bwd
+
+    q = torch.zeros(4, 2, 64, dtype=BF)
+    with pytest.raises(ValueError):
+        attention(q, q, q)
+    with pytest.raises(ValueError):
+        attention_bwd(q, q, q, q, q, torch.zeros(2, 4))
+
+
+def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
+    from megray_b200 import _lib
+
+    lib = _lib.load()
+    t = _lib.AttnTensor(1024, 128, 64)
+    ok = dict(cu=None, dtype=10, tokens=4, heads=2, kv_heads=1, dim=64, seqs=1, causal=1, scale=1.0, error_flag=None)
+    fwd = lambda a, *ts: lib.megray_attention(a, *ts, 1024, None)  # noqa: E731
+    assert fwd(None, t, t, t, t) == 6
+    for bad in (dict(dtype=7), dict(tokens=-1), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(dim=0), dict(dim=60),
+                dict(dim=136), dict(seqs=-1), dict(cu=1024, seqs=0), dict(cu=1025), dict(scale=0.0), dict(scale=float("nan")),
+                dict(scale=float("inf"))):
+        assert fwd(_lib.AttnArgs(**{**ok, **bad}), t, t, t, t) in (6, -1), bad
+    a = _lib.AttnArgs(**ok)
+    for bad in (_lib.AttnTensor(None, 128, 64), _lib.AttnTensor(1032, 128, 64), _lib.AttnTensor(1024, 124, 64),
+                _lib.AttnTensor(1024, 128, 60), _lib.AttnTensor(1024, 0, 64), _lib.AttnTensor(1024, -128, 64), None):
+        for i in range(4):
+            ts = [t] * 4
+            ts[i] = bad
+            assert fwd(a, *ts) == -1
+    assert lib.megray_attention(a, t, t, t, t, None, None) == -1
+    assert lib.megray_attention_bwd(a, t, t, t, t, t, None, t, t, t, 1024, None) == -1
+    assert lib.megray_attention_bwd(a, t, t, t, t, t, 1024, t, t, t, None, None) == -1
+    assert fwd(_lib.AttnArgs(**{**ok, "tokens": 0}), t, t, t, t) == 0
