@@ -225,10 +225,11 @@ int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_ada
 
 /* Balance loss of a router (src/kernels/balance.cuh): loss = coef * experts * sum_e f[e] P[e] with the share f of
  * the counted pairs and the mean probability P of every expert, pairs per expert, and the gradient of the logits.
- * megray_balance makes at most two launches; `workspace` holds megray_balance_workspace(tokens, experts) bytes.  The two
- * halves apart, for partial sums that are added up over ranks in between: megray_balance_stats writes
- * megray_balance_partials(tokens, experts) records of megray_balance_record(experts) bytes (float sums[experts], int32
- * counts[experts], int32 tokens), megray_balance_grad reads `n_partials` of them. */
+ * megray_balance makes at most two launches; `workspace` holds megray_balance_workspace(tokens, experts) bytes, 16-byte
+ * aligned.  The two halves apart, for partial sums that are added up over ranks in between: megray_balance_stats begins
+ * the workspace with megray_balance_partials(tokens, experts) records of megray_balance_record(experts) bytes (float
+ * sums[experts], int32 counts[experts], int32 tokens); megray_balance_grad reads `n_partials` records and the rest of
+ * that workspace. */
 typedef struct {
     const void* logits;    /* [tokens, experts], rows `ld` elements apart */
     const void* idx;       /* [tokens, top] contiguous; entries outside [0, experts) are not counted */
@@ -248,8 +249,9 @@ typedef struct {
 size_t megray_balance_workspace(int tokens, int experts);
 int megray_balance_partials(int tokens, int experts);
 size_t megray_balance_record(int experts);
-int megray_balance_stats(const megray_router* r, void* partials, void* stream);
-int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const megray_balance_out* out, void* stream);
+int megray_balance_stats(const megray_router* r, void* workspace, void* stream);
+int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const void* workspace,
+                        const megray_balance_out* out, void* stream);
 int megray_balance(const megray_router* r, const megray_balance_out* out, void* workspace, void* stream);
 
 /* ---- one pass of the single-GPU models -----------------------------------------------------------

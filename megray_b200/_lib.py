@@ -198,7 +198,7 @@ def _declare(lib) -> None:
     d("megray_balance_partials", i32, i32, i32)
     d("megray_balance_record", sz, i32)
     d("megray_balance_stats", i32, P(Router), vp, vp)
-    d("megray_balance_grad", i32, P(Router), vp, i32, P(BalanceOut), vp)
+    d("megray_balance_grad", i32, P(Router), vp, i32, vp, P(BalanceOut), vp)
     d("megray_balance", i32, P(Router), P(BalanceOut), vp, vp)
     d("megray_tp_ag_gemm", i32, vp, P(GemmArgs), vp, vp, vp, vp)
     d("megray_tp_gemm_rs", i32, vp, P(GemmArgs), vp, vp, vp, vp, C.c_size_t, vp)

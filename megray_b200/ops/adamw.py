@@ -21,6 +21,11 @@ _CODES = {torch.float32: 7, torch.bfloat16: 10}
 _RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("copy", "u8"), ("n", "u8"), ("block", "u8")])
 
 
+# (called once per tensor: as C functions on a list, which is what a long one costs on the host)
+_dtype, _numel, _device = torch.Tensor.dtype.__get__, torch.Tensor.numel, torch.Tensor.get_device
+_contiguous, _address = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
 class AdamWState:
     """Moments of ``params`` (CUDA tensors of one device), zero at first.
 
@@ -106,30 +111,27 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
         args.m_scale = _buffer(state.m_scale, total // BLOCK, torch.float32, device, "m_scale")
         args.v_scale = _buffer(state.r_scale, total // BLOCK, torch.float32, device, "r_scale")
 
-    records = state._records
+    records, sizes = state._records, state.sizes
     keep = [i for i, g in enumerate(grads) if g is not None]
     if len(keep) < n:
         params, grads = [params[i] for i in keep], [grads[i] for i in keep]
         copies = [copies[i] for i in keep] if copies is not None else None
-        records = records[keep]
-    sizes = records["n"].tolist()
-    index = device.index
-    for name, ts, types in (("parameter", params, _CODES), ("gradient", grads, _CODES),
-                            ("copy", copies or [], (torch.bfloat16,))):
-        kinds = {t.dtype for t in ts}
+        records, sizes = records[keep], [sizes[i] for i in keep]
+    records = records.copy()
+    for name, field, ts, types in (("parameter", "p", params, _CODES), ("gradient", "g", grads, _CODES),
+                                   ("copy", "copy", copies or [], (torch.bfloat16,))):
+        if not ts:
+            continue
+        kinds = set(map(_dtype, ts))
         if not kinds.issubset(types):
             raise ValueError(f"adamw_step: a {name} is {kinds}; float32 and bf16 are taken, bf16 alone for copies")
-        if ts and ([t.numel() for t in ts] != sizes or {t.get_device() for t in ts} != {index} or
-                   not all([t.is_contiguous() for t in ts])):
+        if (list(map(_numel, ts)) != sizes or set(map(_device, ts)) != {device.index} or
+                not all(map(_contiguous, ts))):
             raise ValueError(f"adamw_step: a {name} has another size than its parameter had when the state was made, "
                              "is not contiguous or lies on another device")
-    records = records.copy()
-    records["p"] = [t.data_ptr() for t in params]
-    records["g"] = [t.data_ptr() for t in grads]
-    if copies is not None:
-        records["copy"] = [t.data_ptr() for t in copies]
+        records[field] = np.fromiter(map(_address, ts), dtype=np.uint64, count=len(ts))
     lib, stream = _lib.load(), raw_stream()
-    kinds = {(p.dtype, g.dtype) for p, g in zip(params, grads)}
+    kinds = set(zip(map(_dtype, params), map(_dtype, grads)))
     for kind in kinds:
         part = records
         if len(kinds) > 1:

@@ -73,19 +73,18 @@ def balance_loss_grad(logits: torch.Tensor, idx: torch.Tensor, coef: float, *, m
     out, loss, counts, dlogits = _out(logits, coef, dlogits, accumulate)
     lib, stream = _lib.load(), raw_stream()
     tokens, experts = logits.shape
+    room = torch.empty(lib.megray_balance_workspace(tokens, experts), dtype=torch.uint8, device=logits.device)
     if comm is None or comm.nranks == 1:
-        room = torch.empty(lib.megray_balance_workspace(tokens, experts), dtype=torch.uint8, device=logits.device)
         rc = lib.megray_balance(router, out, room.data_ptr(), stream)
         if rc != 0:
             raise RuntimeError(f"megray_balance failed ({rc})")
         return loss, counts, dlogits
-    n, words = lib.megray_balance_partials(tokens, experts), lib.megray_balance_record(experts) // 4
-    part = torch.empty(n, words, dtype=torch.int32, device=logits.device)
-    rc = lib.megray_balance_stats(router, part.data_ptr(), stream)
+    n, size = lib.megray_balance_partials(tokens, experts), lib.megray_balance_record(experts)
+    rc = lib.megray_balance_stats(router, room.data_ptr(), stream)
     if rc != 0:
         raise RuntimeError(f"megray_balance_stats failed ({rc})")
-    total = add_ranks(comm, part, experts)
-    rc = lib.megray_balance_grad(router, total.data_ptr(), 1, out, stream)
+    total = add_ranks(comm, room[:n * size].view(torch.int32).view(n, size // 4), experts)
+    rc = lib.megray_balance_grad(router, total.data_ptr(), 1, room.data_ptr(), out, stream)
     if rc != 0:
         raise RuntimeError(f"megray_balance_grad failed ({rc})")
     return loss, counts, dlogits

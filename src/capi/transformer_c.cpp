@@ -82,36 +82,33 @@ int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_ada
 
 int megray_balance_partials(int tokens, int experts) { return mgk::balance::partials(tokens, experts); }
 size_t megray_balance_record(int experts) { return static_cast<size_t>(mgk::balance::partial_words(experts)) * 4; }
-size_t megray_balance_workspace(int tokens, int experts) {
-    return mgk::balance::partials(tokens, experts) * megray_balance_record(experts);
-}
-int megray_balance_stats(const megray_router* r, void* partials, void* stream) {
+size_t megray_balance_workspace(int tokens, int experts) { return mgk::balance::workspace_bytes(tokens, experts); }
+int megray_balance_stats(const megray_router* r, void* workspace, void* stream) {
     mgk::balance::Router router;
     if (!to_router(r, &router))
         return kInvalid;
-    return rc(mgk::balance::launch_stats(router, partials, S(stream)));
+    return rc(mgk::balance::launch_stats(router, workspace, S(stream)));
 }
-int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const megray_balance_out* out,
-                        void* stream) {
+int megray_balance_grad(const megray_router* r, const void* partials, int n_partials, const void* workspace,
+                        const megray_balance_out* out, void* stream) {
     mgk::balance::Router router;
     mgk::balance::Result result;
     if (!to_router(r, &router) || !to_result(out, &result))
         return kInvalid;
-    return rc(mgk::balance::launch_grad(router, partials, n_partials, result, S(stream)));
+    return rc(mgk::balance::launch_grad(router, partials, n_partials, workspace, result, false, S(stream)));
 }
 int megray_balance(const megray_router* r, const megray_balance_out* out, void* workspace, void* stream) {
     mgk::balance::Router router;
     mgk::balance::Result result;
     if (!to_router(r, &router) || !to_result(out, &result))
         return kInvalid;
-    const cudaError_t one = mgk::balance::launch_small(router, result, S(stream));
-    if (one != cudaErrorNotSupported)
-        return rc(one);
+    if (mgk::balance::is_small(router.tokens, router.experts))
+        return rc(mgk::balance::launch_small(router, workspace, result, S(stream)));
     const cudaError_t e = mgk::balance::launch_stats(router, workspace, S(stream));
     if (e != cudaSuccess)
         return rc(e);
-    return rc(mgk::balance::launch_grad(router, workspace, mgk::balance::partials(router.tokens, router.experts), result,
-                                        S(stream)));
+    return rc(mgk::balance::launch_grad(router, workspace, mgk::balance::partials(router.tokens, router.experts), workspace,
+                                        result, true, S(stream)));
 }
 
 }  // extern "C"

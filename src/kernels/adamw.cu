@@ -3,10 +3,6 @@
 //   m <- b1 m + (1 - b1) g        v <- b2 v + (1 - b2) g^2        (g times grad_scale)
 //   p <- p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v / (1 - b2^t)) + eps)
 //
-// Every operation is rounded on its own (no contraction into fused multiply-adds), so that the update is
-// the one that a list of elementary float32 operations gives, bit for bit, on any split of the work: an 8-bit
-// moment next to the border of two numbers falls to the same side.
-//
 // 8-bit moments: blocks of 256 elements of one tensor hold m and r = sqrt(v) as e4m3 numbers times a
 // float32 scale, the block's largest magnitude over 448.  The root and not v itself: e4m3 spans 2^18, which is
 // 2^36 of v, and its half step of 2^-4 then is one of the denominator too.  A root that is not zero is never
@@ -14,8 +10,16 @@
 // kept between steps is rounded.  A NaN or an infinity in a block's gradients makes the block's scale NaN or
 // infinite and with it the block.
 //
-// Bound by HBM.  A warp takes one block of 256 elements, eight a lane, so a scale is found with one
-// warp-wide integer maximum (float magnitudes order as integers, NaN above all) and nothing is read twice.
+// Moments are formed with every operation rounded on its own, in the order of the formulas (no contraction into fused
+// multiply-adds): they are those of a list of elementary float32 operations bit for bit, so that an
+// 8-bit moment next to the border of two numbers falls to the same side everywhere.  The update itself, which is not
+// kept in 8 bits, uses the hardware's approximate reciprocal, a few float32 steps off.
+//
+// Bound by HBM, with the issue slots close behind: 10 bytes an element with 8-bit moments and bf16 tensors leave
+// about 55 instructions for it; products and sums are issued in pairs.  A warp takes blocks of 256 elements, two
+// runs of four a lane so that every access of the warp is contiguous whatever the types, and loads the next block
+// before it works on one (latency, not bandwidth, was the limit without: 40 M elements 97 us).  A scale is found with
+// one warp-wide integer maximum (float magnitudes order as integers, NaN above all) and nothing is read twice.
 // Tensors' addresses travel as kernel parameters: no copy to the device before the launch, and a captured
 // graph replays them.
 #include "adamw.cuh"
@@ -35,9 +39,9 @@ namespace adamw {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerCta = kThreads / 32;
-constexpr float kTop = 448.f;          // largest e4m3 number
-constexpr float kLeast = 0x1p-100f;    // a block whose largest magnitude is below is kept as zeros
+constexpr int kWarps = kThreads / 32;
+constexpr float kTop = 448.f;        // largest e4m3 number
+constexpr float kLeast = 0x1p-100f;  // a block whose largest magnitude is below is kept as zeros
 
 struct Entry {
     void* p;
@@ -52,6 +56,7 @@ struct Table {
     Entry e[CAP];
     uint32_t first_cta[CAP];
     int count;
+    int per_warp;  // blocks that a warp takes, kWarps apart
 };
 
 struct Args {
@@ -62,104 +67,194 @@ struct Args {
     double lr, beta1, beta2, weight_decay, step;
 };
 
-__device__ __forceinline__ void load8(const float* s, float (&f)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4*>(s)), b = __ldcs(reinterpret_cast<const float4*>(s) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* s, float (&f)[8]) {
-    const uint4 a = __ldcs(reinterpret_cast<const uint4*>(s));
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-__device__ __forceinline__ void store8(float* d, const float (&f)[8]) {
-    reinterpret_cast<float4*>(d)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(d)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* d, const float (&f)[8]) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(float* d, float x) { *d = x; }
-__device__ __forceinline__ void put(__nv_bfloat16* d, float x) { *d = __float2bfloat16_rn(x); }
-
-// Eight values of a lane, the whole vector where it may be read as one, else one by one up to `live`
+// A lane's eight elements are [4 lane, 4 lane + 4) and [128 + 4 lane, ...) of its warp's block.  They are loaded as
+// words, float32 one and bf16 two to a word.
 template <class T>
-__device__ __forceinline__ void load_some(const T* s, bool whole, int live, float (&f)[8]) {
+constexpr int words_of() { return static_cast<int>(2 * sizeof(T)); }
+
+__device__ __forceinline__ uint32_t bits_of(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 x) { return __bfloat16_as_ushort(x); }
+
+// As vectors where the block's address and length allow it, else one by one; `live` counts the elements from the
+// lane's first on
+template <class T>
+__device__ __forceinline__ void load_words(const T* s, bool whole, int live, uint32_t (&w)[words_of<T>()]) {
     if (whole) {
-        load8(s, f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (sizeof(T) == 4) {
+                const uint4 a = __ldcs(reinterpret_cast<const uint4*>(s + 128 * h));
+                w[4 * h] = a.x; w[4 * h + 1] = a.y; w[4 * h + 2] = a.z; w[4 * h + 3] = a.w;
+            } else {
+                const uint2 a = __ldcs(reinterpret_cast<const uint2*>(s + 128 * h));
+                w[2 * h] = a.x; w[2 * h + 1] = a.y;
+            }
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            f[i] = i < live ? to_float(s[i]) : 0.f;
+        for (int i = 0; i < words_of<T>(); ++i)
+            w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int at = (i >> 2) * 128 + (i & 3);
+            if (at < live)
+                w[i * words_of<T>() / 8] |= bits_of(s[at]) << (sizeof(T) == 4 ? 0 : 16 * (i & 1));
+        }
     }
+}
+template <class T>
+__device__ __forceinline__ void unpack(const uint32_t (&w)[words_of<T>()], float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 4)
+            f[i] = __uint_as_float(w[i]);
+        else
+            f[i] = __uint_as_float((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+}
+__device__ __forceinline__ void put(float* d, float x) { *d = x; }
+__device__ __forceinline__ void put(__nv_bfloat16* d, float x) { *d = __float2bfloat16_rn(x); }
+__device__ __forceinline__ void store4(float* d, const float* f) {
+    *reinterpret_cast<float4*>(d) = make_float4(f[0], f[1], f[2], f[3]);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* d, const float* f) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
+    *reinterpret_cast<uint2*>(d) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
 }
 template <class T>
 __device__ __forceinline__ void store_some(T* d, bool whole, int live, const float (&f)[8]) {
     if (whole) {
-        store8(d, f);
+        store4(d, f);
+        store4(d + 128, f + 4);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < live)
-                put(d + i, f[i]);
+        for (int i = 0; i < 8; ++i) {
+            const int at = (i >> 2) * 128 + (i & 3);
+            if (at < live)
+                put(d + at, f[i]);
+        }
     }
 }
 template <class T>
 __device__ __forceinline__ bool vector_ok(const T* p) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+    return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
 }
 
-__device__ __forceinline__ void decode8(uint2 code, float scale, float (&f)[8]) {
-    const uint32_t w[2] = {code.x, code.y};
+// Two float32 products in one instruction, each rounded on its own
+struct Pair {
+    float x, y;
+};
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+    Pair d;
+    asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n mul.rn.f32x2 r, p, q;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// (one by one: a paired sum of paired products was contracted into fused multiply-adds)
+__device__ __forceinline__ Pair add(Pair a, Pair b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{\n .reg .b64 p, q, r, s;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n mov.b64 r, {%6, %7};\n"
+        " fma.rn.f32x2 s, p, q, r;\n mov.b64 {%0, %1}, s;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ Pair both(float x) { return {x, x}; }
+
+// four e4m3 numbers times a scale
+__device__ __forceinline__ void decode4(uint32_t code, float scale, float* f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i >> 1] >> (16 * (i & 1))),
-                                                         __NV_E4M3);
+    for (int i = 0; i < 2; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(code >> (16 * i)), __NV_E4M3);
         const float2 x = __half22float2(__half2(h));
-        f[2 * i] = __fmul_rn(x.x, scale);
-        f[2 * i + 1] = __fmul_rn(x.y, scale);
+        const Pair y = mul({x.x, x.y}, both(scale));
+        f[2 * i] = y.x;
+        f[2 * i + 1] = y.y;
     }
 }
-__device__ __forceinline__ uint32_t warp_top(const float (&f)[8]) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-    return __reduce_max_sync(0xffffffffu, top);
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
-// e4m3 numbers of f over the block's scale, which is returned too
-template <bool KEEP>
-__device__ __forceinline__ uint2 encode8(const float (&f)[8], float& scale) {
-    const float top = __uint_as_float(warp_top(f));
-    const float inv = top < kLeast ? 0.f : __fmul_rn(__frcp_rn(top), kTop);
-    scale = top < kLeast ? 0.f : __fmul_rn(top, 1.f / kTop);
-    uint32_t w[4];
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// the larger magnitude of a and those of b and c; a NaN is kept
+__device__ __forceinline__ float top_of(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+    return d;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Square roots of eight numbers, exact but for a few in a million that are one float32 step off: the approximate
+// reciprocal root and one correction by the exact residual.  Zeros, numbers near the denormal ones and infinities
+// take CUDA's function.
+__device__ __forceinline__ void roots8(const float (&v)[8], float (&r)[8]) {
+    const float lo = fminf(min3(v[0], v[1], v[2]), fminf(min3(v[3], v[4], v[5]), fminf(v[6], v[7])));
+    const float hi = fmaxf(max3(v[0], v[1], v[2]), fmaxf(max3(v[3], v[4], v[5]), fmaxf(v[6], v[7])));
+    if (lo >= 0x1p-100f && hi <= 0x1p100f) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float a = __fmul_rn(f[2 * i], inv), b = __fmul_rn(f[2 * i + 1], inv);
-        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        if (KEEP) {
-            w[i] |= (w[i] & 0xffu) == 0 && f[2 * i] > 0.f ? 1u : 0u;
-            w[i] |= (w[i] & 0xff00u) == 0 && f[2 * i + 1] > 0.f ? 0x100u : 0u;
+        for (int i = 0; i < 8; i += 2) {
+            Pair y;
+            asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(v[i]));
+            asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(v[i + 1]));
+            const Pair x{v[i], v[i + 1]}, s = mul(x, y);
+            const Pair q = fma(fma({-s.x, -s.y}, s, x), mul(y, both(0.5f)), s);
+            r[i] = q.x;
+            r[i + 1] = q.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            r[i] = __fsqrt_rn(v[i]);
+    }
+}
+// e4m3 numbers of a block over its scale, which is returned
+template <bool KEEP>
+__device__ __forceinline__ float encode8(const float (&f)[8], uint32_t (&code)[2]) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+        t = top_of(t, f[i], f[i + 1]);
+    const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(t)));
+    const float inv = top < kLeast ? 0.f : __fmul_rn(__frcp_rn(top), kTop);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float* x = f + 4 * i;
+        const Pair y = mul({x[0], x[1]}, both(inv)), z = mul({x[2], x[3]}, both(inv));
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y.x, y.y), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(z.x, z.y), __NV_SATFINITE, __NV_E4M3);
+        code[i] = lo | (hi << 16);
+        // seldom: a number that came out as zero
+        if (KEEP && ((code[i] - 0x01010101u) & ~code[i] & 0x80808080u) != 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (((code[i] >> (8 * k)) & 0xffu) == 0 && x[k] > 0.f)
+                    code[i] |= 1u << (8 * k);
         }
     }
-    return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+    return top < kLeast ? 0.f : __fmul_rn(top, 1.f / kTop);
 }
 
+// What a lane reads of a block
+template <class P, class G, int BITS>
+struct Raw {
+    static constexpr int MW = BITS == 8 ? 2 : 8;
+    uint32_t p[words_of<P>()], g[words_of<G>()], m[MW], v[MW];
+    float sm, sv;
+};
+
 template <class P, class G, int BITS, int CAP>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ Table<CAP> t, const Args a) {
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? 4 : 3) adamw_kernel(const __grid_constant__ Table<CAP> t, const Args a) {
     __shared__ float from_device[3];
     float keep = a.keep, rate = a.rate, root = a.root, grad_scale = a.grad_scale;
     if (a.lr_dev != nullptr || a.step_dev != nullptr || a.grad_scale_dev != nullptr) {
@@ -187,71 +282,125 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
             hi = mid;
     }
     const Entry& e = t.e[lo];
-    const uint64_t block = static_cast<uint64_t>(blockIdx.x - t.first_cta[lo]) * kBlocksPerCta + (threadIdx.x >> 5);
-    if (block * kBlock >= e.n)
-        return;
     const int lane = threadIdx.x & 31;
-    const uint64_t at = block * kBlock + lane * 8;
-    const int live = at >= e.n ? 0 : static_cast<int>(min(static_cast<uint64_t>(8), e.n - at));
-    const bool full = live == 8;
-    P* pp = static_cast<P*>(e.p) + at;
-    const G* gp = static_cast<const G*>(e.g) + at;
-    const uint64_t sb = e.block + block;           // block in the moment buffers
-    const uint64_t sat = sb * kBlock + lane * 8;
+    // from the CTA's first element on everything fits 32 bits
+    const uint64_t cta_block = static_cast<uint64_t>(blockIdx.x - t.first_cta[lo]) * (kWarps * t.per_warp);
+    const uint64_t cta_at = cta_block * kBlock, sb0 = e.block + cta_block;
+    const int n = static_cast<int>(min(e.n - cta_at, static_cast<uint64_t>(kBlock * kWarps * t.per_warp)));
+    P* const p0 = static_cast<P*>(e.p) + cta_at;
+    const G* const g0 = static_cast<const G*>(e.g) + cta_at;
+    __nv_bfloat16* const c0 = e.copy != nullptr ? static_cast<__nv_bfloat16*>(e.copy) + cta_at : nullptr;
+    using M = typename std::conditional<BITS == 8, uint8_t, float>::type;
+    M* const m0 = static_cast<M*>(a.m) + sb0 * kBlock;
+    M* const v0 = static_cast<M*>(a.v) + sb0 * kBlock;
+    const bool p_ok = vector_ok(p0), g_ok = vector_ok(g0), c_ok = vector_ok(c0);
+    const Pair gs = both(grad_scale), b1 = both(a.b1), c1 = both(a.c1), b2 = both(a.b2), c2 = both(a.c2);
 
-    float p[8], g[8], m[8], v[8];
-    load_some(pp, full && vector_ok(pp), live, p);
-    load_some(gp, full && vector_ok(gp), live, g);
-    if (BITS == 8) {
-        decode8(__ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.m) + sat)), a.m_scale[sb], m);
-        decode8(__ldcs(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.v) + sat)), a.v_scale[sb], v);
+    auto load = [&](int block, Raw<P, G, BITS>& r) {
+        const int at = block * kBlock + lane * 4, live = n - at;
+        const bool full = block * kBlock + kBlock <= n;  // (the same in all lanes)
+        load_words(p0 + at, full && p_ok, live, r.p);
+        load_words(g0 + at, full && g_ok, live, r.g);
+        if constexpr (BITS == 8) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = __fmul_rn(v[i], v[i]);
-    } else {
-        load8(static_cast<const float*>(a.m) + sat, m);
-        load8(static_cast<const float*>(a.v) + sat, v);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = __fmul_rn(g[i], grad_scale);
-        m[i] = __fadd_rn(__fmul_rn(m[i], a.b1), __fmul_rn(x, a.c1));
-        v[i] = __fadd_rn(__fmul_rn(v[i], a.b2), __fmul_rn(__fmul_rn(x, x), a.c2));
-        const float r = __fsqrt_rn(v[i]);
-        const float u = __fdiv_rn(m[i], __fadd_rn(__fmul_rn(r, root), a.eps));
-        p[i] = __fsub_rn(__fmul_rn(p[i], keep), __fmul_rn(u, rate));
-        if (BITS == 8)
-            v[i] = r;
-    }
-    store_some(pp, full && vector_ok(pp), live, p);
-    if (e.copy != nullptr) {
-        __nv_bfloat16* cp = static_cast<__nv_bfloat16*>(e.copy) + at;
-        store_some(cp, full && vector_ok(cp), live, p);
-    }
-    if (BITS == 8) {
-        float sm, sr;
-        const uint2 cm = encode8<false>(m, sm), cr = encode8<true>(v, sr);
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.m) + sat) = cm;
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.v) + sat) = cr;
-        if (lane == 0) {
-            a.m_scale[sb] = sm;
-            a.v_scale[sb] = sr;
+            for (int h = 0; h < 2; ++h) {
+                r.m[h] = __ldcs(reinterpret_cast<const uint32_t*>(m0 + at + 128 * h));
+                r.v[h] = __ldcs(reinterpret_cast<const uint32_t*>(v0 + at + 128 * h));
+            }
+            r.sm = a.m_scale[sb0 + block];
+            r.sv = a.v_scale[sb0 + block];
+        } else {
+            load_words(m0 + at, true, 0, r.m);
+            load_words(v0 + at, true, 0, r.v);
         }
-    } else {
-        store8(static_cast<float*>(a.m) + sat, m);
-        store8(static_cast<float*>(a.v) + sat, v);
+    };
+
+    Raw<P, G, BITS> raw;
+    const int first = threadIdx.x >> 5;
+    if (first * kBlock < n)
+        load(first, raw);
+#pragma unroll 1
+    for (int block = first; block * kBlock < n; block += kWarps) {
+        float p[8], g[8], m[8], v[8];
+        unpack<P>(raw.p, p);
+        unpack<G>(raw.g, g);
+        if constexpr (BITS == 8) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                decode4(raw.m[h], raw.sm, m + 4 * h);
+                decode4(raw.v[h], raw.sv, v + 4 * h);
+            }
+        } else {
+            unpack<float>(raw.m, m);
+            unpack<float>(raw.v, v);
+        }
+        if ((block + kWarps) * kBlock < n)
+            load(block + kWarps, raw);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            Pair mm{m[i], m[i + 1]}, vv{v[i], v[i + 1]};
+            if (BITS == 8)
+                vv = mul(vv, vv);
+            const Pair x = mul({g[i], g[i + 1]}, gs);
+            mm = add(mul(mm, b1), mul(x, c1));
+            vv = add(mul(vv, b2), mul(mul(x, x), c2));
+            m[i] = mm.x;
+            m[i + 1] = mm.y;
+            v[i] = vv.x;
+            v[i + 1] = vv.y;
+        }
+        float r[8];
+        roots8(v, r);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const Pair d = fma({r[i], r[i + 1]}, both(root), both(a.eps));
+            const Pair u = mul({m[i], m[i + 1]}, {rcp_approx(d.x), rcp_approx(d.y)});
+            const Pair q = fma(u, both(-rate), mul({p[i], p[i + 1]}, both(keep)));
+            p[i] = q.x;
+            p[i + 1] = q.y;
+        }
+        const int at = block * kBlock + lane * 4, live = n - at;
+        const bool full = block * kBlock + kBlock <= n;
+        store_some(p0 + at, full && p_ok, live, p);
+        if (c0 != nullptr)
+            store_some(c0 + at, full && c_ok, live, p);
+        if constexpr (BITS == 8) {
+            uint32_t code[2];
+            const float sm = encode8<false>(m, code);
+            uint32_t* to = reinterpret_cast<uint32_t*>(m0 + at);
+            to[0] = code[0];
+            to[32] = code[1];
+            const float sv = encode8<true>(r, code);
+            to = reinterpret_cast<uint32_t*>(v0 + at);
+            to[0] = code[0];
+            to[32] = code[1];
+            if (lane == 0) {
+                a.m_scale[sb0 + block] = sm;
+                a.v_scale[sb0 + block] = sv;
+            }
+        } else {
+            store_some(m0 + at, true, 0, m);
+            store_some(v0 + at, true, 0, v);
+        }
     }
 }
 
 template <class P, class G, int BITS, int CAP>
 cudaError_t launch_table(const Tensor* tensors, int count, const Args& a, cudaStream_t stream) {
     Table<CAP> t;
+    uint64_t blocks = 0;
+    for (int k = 0; k < count; ++k)
+        blocks += (tensors[k].n + kBlock - 1) / kBlock;
+    // four blocks a warp once that still fills the chip three times over (what a warp does once, finding its
+    // tensor above all, costs as many instructions as a block), else one, for the shortest way through
+    t.per_warp = blocks >= 148ull * 3 * kWarps * 12 ? 4 : 1;
+    const uint64_t chunk = static_cast<uint64_t>(kBlock) * kWarps * t.per_warp;
     int i = 0;
     while (i < count) {
         uint64_t ctas = 0;
         t.count = 0;
         for (; i < count && t.count < CAP; ++i) {
-            const uint64_t need = (tensors[i].n + kBlock * kBlocksPerCta - 1) / (kBlock * kBlocksPerCta);
+            const uint64_t need = (tensors[i].n + chunk - 1) / chunk;
             if (need == 0)
                 continue;
             if (need > 0x7fffffffull)

@@ -7,12 +7,14 @@
 // (f has no gradient; a constant taken off f leaves the gradient as it is, since the p of a row add up to one,
 // and without it the difference would cancel to a few digits where the experts are evenly used.)
 //
-// Two passes over the logits, since the gradient of every token needs the sums over all of them.  Bound by
-// memory or by launches.  A group of W lanes holds a row in registers, W the power of two that covers it,
-// up to a warp, so that short rows share a warp.  The sums are formed without floating-point atomics: lanes over
-// their rows, warps of a CTA in order, CTAs of a cluster in order through distributed shared memory, clusters in
-// order by the second kernel: the same bits in every run.  Problems that one cluster of eight CTAs can do in a few
-// microseconds take one launch, the cluster's barrier between the passes.
+// Two passes over the logits, since the gradient of every token needs the sums over all of them; the first leaves
+// every row's maximum and reciprocal sum behind (8 bytes a row), so that the second has one sum over a row to
+// form.  Bound by memory or by launches.  A group of W lanes holds a row in registers, W the power of two that covers
+// it, up to a warp, so that short rows share a warp; a warp has several rows in flight.  The sums are
+// formed without floating-point atomics: lanes over their rows, warps of a CTA in order, CTAs of a cluster in order
+// through distributed shared memory, clusters in order by the second kernel: the same bits in every run.  The
+// second kernel's clusters share the work of adding the partial sums up.  Problems that one cluster of eight CTAs
+// can do in a few microseconds take one launch, the cluster's barrier between the passes.
 #include "balance.cuh"
 
 #include <cooperative_groups.h>
@@ -31,155 +33,304 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
 
-__device__ __forceinline__ float at(const float* p) { return *p; }
-__device__ __forceinline__ float at(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
-
 template <int VEC>
 __device__ __forceinline__ void load_vec(const float* p, float (&f)[VEC]) {
-    if (VEC == 4) {
+    static_assert(VEC == 4 || VEC == 1, "16 bytes or one element");
+    if constexpr (VEC == 4) {
         const float4 v = *reinterpret_cast<const float4*>(p);
-        f[0] = v.x; f[1 % VEC] = v.y; f[2 % VEC] = v.z; f[3 % VEC] = v.w;
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
     } else {
         f[0] = *p;
     }
 }
 template <int VEC>
 __device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&f)[VEC]) {
-    if (VEC == 4) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        f[0] = __uint_as_float(v.x << 16); f[1 % VEC] = __uint_as_float(v.x & 0xffff0000u);
-        f[2 % VEC] = __uint_as_float(v.y << 16); f[3 % VEC] = __uint_as_float(v.y & 0xffff0000u);
-    } else {
+    static_assert(VEC == 8 || VEC == 4 || VEC == 1, "16 or 8 bytes or one element");
+    if constexpr (VEC == 1) {
         f[0] = __bfloat162float(*p);
+    } else {
+        uint32_t w[VEC / 2];
+        if constexpr (VEC == 8)
+            *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+        else
+            *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            f[2 * i] = __uint_as_float(w[i] << 16);
+            f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
     }
+}
+// (float32 gradients beside bf16 logits are stored eight elements at a time too)
+template <int VEC>
+__device__ __forceinline__ void load_old(const float* p, float (&f)[VEC]) {
+    if constexpr (VEC == 8) {
+        float lo[4], hi[4];
+        load_vec<4>(p, lo);
+        load_vec<4>(p + 4, hi);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f[i] = lo[i];
+            f[4 + i] = hi[i];
+        }
+    } else {
+        load_vec<VEC>(p, f);
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void load_old(const __nv_bfloat16* p, float (&f)[VEC]) {
+    load_vec<VEC>(p, f);
 }
 template <int VEC>
 __device__ __forceinline__ void store_vec(float* p, const float (&f)[VEC]) {
-    if (VEC == 4)
-        *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1 % VEC], f[2 % VEC], f[3 % VEC]);
-    else
+    if constexpr (VEC == 1) {
         *p = f[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4)
+            *reinterpret_cast<float4*>(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+    }
 }
 template <int VEC>
 __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&f)[VEC]) {
-    if (VEC == 4) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1 % VEC]), b = __floats2bfloat162_rn(f[2 % VEC], f[3 % VEC]);
-        *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    } else {
+    if constexpr (VEC == 1) {
         *p = __float2bfloat16_rn(f[0]);
+    } else {
+        uint32_t w[VEC / 2];
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if constexpr (VEC == 8)
+            *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(w);
+        else
+            *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(w);
     }
 }
 
-// One row over W lanes: x becomes the probabilities of its columns (zero beyond the last one).  A row
-// that holds nothing but -infinity has no probabilities.
+// Rows that a group of lanes has in flight: 16 registers of logits where a row takes fewer
 template <int VEC, int NC>
-__device__ __forceinline__ void softmax_row(float (&x)[NC][VEC], int W) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            top = fmaxf(top, x[i][v]);
-    for (int o = W >> 1; o > 0; o >>= 1)
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (top == -INFINITY)
-        top = 0.f;
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            x[i][v] = __expf(x[i][v] - top);
-            sum += x[i][v];
-        }
-    for (int o = W >> 1; o > 0; o >>= 1)
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v)
-            x[i][v] *= inv;
+__host__ __device__ constexpr int rows_in_flight() {
+    return VEC * NC >= 16 ? 1 : VEC * NC >= 8 ? 2 : 4;
 }
 
+constexpr float LOG2E = 1.4426950408889634f;
+
+// x <- exp(x - top), with what is below the normal numbers as zero.  One fused step in front of 2^x; its rounding of
+// top log2e is the same in every term of a row and drops out where they are divided by their sum.  Where logits are
+// near the type's lowest number the product with log2e would overflow: there the difference comes first.
+template <int NC, int VEC>
+__device__ __forceinline__ void exponentials(float (&x)[NC][VEC], float top) {
+    const float t = top * LOG2E;
+    if (fabsf(top) < 1e37f) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[i][v]) : "f"(fmaf(x[i][v], LOG2E, -t)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[i][v]) : "f"((x[i][v] - top) * LOG2E));
+    }
+}
+
+// Sums (or maxima) of U values over groups of W lanes, the U chains side by side
+template <int U>
+__device__ __forceinline__ void group_sum(float (&v)[U], int W) {
+    for (int o = W >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] += __shfl_xor_sync(0xffffffffu, v[u], o);
+}
+template <int U>
+__device__ __forceinline__ void group_max(float (&v)[U], int W) {
+    if (W == 32) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v[u]));
+        return;
+    }
+    for (int o = W >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            v[u] = fmaxf(v[u], __shfl_xor_sync(0xffffffffu, v[u], o));
+}
+
+// A lane's part of a row as words: one element, or 8 or 16 bytes; what is not there is -infinity
+template <class T, int VEC>
+constexpr int words_of() { return VEC == 1 ? 1 : static_cast<int>(VEC * sizeof(T) / 4); }
 template <class T, int VEC, int NC>
-__device__ __forceinline__ void load_row(const T* row, int W, int sub, int experts, float (&x)[NC][VEC]) {
+__device__ __forceinline__ void load_row(const T* row, bool live, int W, int sub, int experts,
+                                         uint32_t (&w)[NC][words_of<T, VEC>()]) {
+    constexpr int N = words_of<T, VEC>();
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         const int c = (i * W + sub) * VEC;
-        if (c < experts) {
-            load_vec<VEC>(row + c, x[i]);
+        if (live && c < experts) {
+            if constexpr (VEC == 1) {
+                w[i][0] = sizeof(T) == 4 ? *reinterpret_cast<const uint32_t*>(row + c)
+                                         : static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + c)) << 16;
+            } else if constexpr (N == 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(row + c);
+                w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(row + c);
+                w[i][0] = v.x; w[i][1] = v.y;
+            }
         } else {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                x[i][v] = -INFINITY;
+            for (int k = 0; k < N; ++k)
+                w[i][k] = sizeof(T) == 4 || VEC == 1 ? 0xff800000u : 0xff80ff80u;
         }
     }
 }
+template <class T, int VEC>
+__device__ __forceinline__ float element(const uint32_t (&w)[words_of<T, VEC>()], int v) {
+    if (sizeof(T) == 4 || VEC == 1)
+        return __uint_as_float(w[v]);
+    return __uint_as_float((v & 1) ? w[v / 2] & 0xffff0000u : w[v / 2] << 16);
+}
 
-// Shared memory of a CTA: float sums [kWarps][E] whose first row becomes the CTA's, int counts [E], int valid,
-// then float w [E] and room for the totals.
+// The rows of a lane: U at a time, 32 / W apart, `left` of them from row `at` on (negative behind the end)
+template <class T, int VEC, int NC>
+struct Walk {
+    static constexpr int U = rows_in_flight<VEC, NC>();
+    const T* p;
+    const uint8_t* mask;
+    int64_t row_step, u_step;
+    int at, left, left_of_warp, step, per_warp;
+
+    __device__ __forceinline__ Walk(const Router& r, int W, int cta, int ctas) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        per_warp = 32 / W;
+        step = ctas * kWarps * per_warp * U;
+        const int first = (cta * kWarps + warp) * per_warp * U;
+        at = first + lane / W;
+        left = r.tokens - at;
+        left_of_warp = r.tokens - first;
+        row_step = step * r.ld;
+        u_step = per_warp * r.ld;
+        p = static_cast<const T*>(r.logits) + at * r.ld;
+        mask = r.mask != nullptr ? r.mask + at : nullptr;
+    }
+    __device__ __forceinline__ bool live(int u) const {
+        return u * per_warp < left && (mask == nullptr || mask[u * per_warp] != 0);
+    }
+    __device__ __forceinline__ const T* row(int u) const { return p + u * u_step; }
+    __device__ __forceinline__ void next() {
+        p += row_step;
+        if (mask != nullptr)
+            mask += step;
+        // (unsigned: the sum may pass the last int once behind the end, where it is not used)
+        at = static_cast<int>(static_cast<uint32_t>(at) + step);
+        left -= step;
+        left_of_warp -= step;
+    }
+};
+
+// Shared memory of a CTA: float sums [kWarps][E] whose first row becomes the CTA's (where the first pass runs) or
+// double totals [E] (where it does not), int counts [E], float w [E], int valid.
 struct Smem {
+    double* total;
     float* sums;
     int* counts;
     int* valid;
     float* w;
-    float* red;
 };
-__device__ __forceinline__ Smem carve(char* base, int experts) {
+__device__ __forceinline__ Smem carve(char* base, int experts, bool sums) {
     Smem s;
+    s.total = reinterpret_cast<double*>(base);
     s.sums = reinterpret_cast<float*>(base);
-    s.counts = reinterpret_cast<int*>(s.sums + kWarps * experts);
-    s.valid = s.counts + experts;
-    s.w = reinterpret_cast<float*>(s.valid + 4);
-    s.red = s.w + experts;
+    s.counts = reinterpret_cast<int*>(base) + (sums ? kWarps : 2) * experts;
+    s.w = reinterpret_cast<float*>(s.counts + experts);
+    s.valid = s.counts + 2 * experts;
     return s;
 }
-size_t smem_bytes(int experts) { return sizeof(float) * (kWarps * experts + experts + 4 + experts + 2 * kWarps + 4); }
+size_t smem_bytes(int experts, bool sums) { return sizeof(float) * (((sums ? kWarps : 2) + 2) * experts + 1); }
 
-// The rows of CTA `cta` of `ctas`: sums over them into s.sums[0..E), s.counts and s.valid.
+// The rows of CTA `cta` of `ctas`: sums over them into s.sums[0..E), s.counts and s.valid, and every row's
+// maximum and reciprocal sum into `rows` (zeros for a row that holds nothing but -infinity: it has no probabilities).
 template <class T, int VEC, int NC>
-__device__ __forceinline__ void cta_stats(const Router& r, int W, int cta, int ctas, const Smem& s) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__device__ __forceinline__ void cta_stats(const Router& r, int W, int cta, int ctas, const Smem& s, float2* rows) {
+    constexpr int U = rows_in_flight<VEC, NC>();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (W - 1), per_warp = 32 / W;
     for (int e = threadIdx.x; e < r.experts; e += kThreads)
         s.counts[e] = 0;
     if (threadIdx.x == 0)
         *s.valid = 0;
     __syncthreads();
-    const int sub = lane & (W - 1), per_warp = 32 / W;
-    const T* logits = static_cast<const T*>(r.logits);
+    // pairs, apart from the rows: contiguous whatever the number per token
+    {
+        const uint32_t pairs = static_cast<uint32_t>(r.tokens) * r.top, by = static_cast<uint32_t>(ctas) * kThreads;
+        for (uint32_t i = static_cast<uint32_t>(cta) * kThreads + threadIdx.x; i < pairs; i += by) {
+            const int64_t e = r.idx64 ? static_cast<const int64_t*>(r.idx)[i] : static_cast<const int*>(r.idx)[i];
+            if (e >= 0 && e < r.experts && (r.mask == nullptr || r.mask[i / static_cast<uint32_t>(r.top)] != 0))
+                atomicAdd(&s.counts[e], 1);
+        }
+    }
     float acc[NC][VEC] = {};
     int valid = 0;
-    const int64_t step = static_cast<int64_t>(ctas) * kWarps * per_warp;
+    Walk<T, VEC, NC> walk(r, W, cta, ctas);
+    uint32_t raw[U][NC][words_of<T, VEC>()];
+    auto load = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool live = walk.live(u);
+            load_row<T, VEC, NC>(walk.row(u), live, W, sub, r.experts, raw[u]);
+            valid += live && sub == 0 ? 1 : 0;
+        }
+    };
+    load();
     // (all lanes of a warp go round alike: the shuffles are warp-wide)
-    for (int64_t base = (static_cast<int64_t>(cta) * kWarps + warp) * per_warp; base < r.tokens; base += step) {
-        const int64_t t = base + lane / W;
-        const bool live = t < r.tokens && (r.mask == nullptr || r.mask[t] != 0);
-        float x[NC][VEC];
-        if (live) {
-            load_row<T, VEC, NC>(logits + t * r.ld, W, sub, r.experts, x);
-            for (int k = sub; k < r.top; k += W) {
-                const int64_t e = r.idx64 ? static_cast<const int64_t*>(r.idx)[t * r.top + k]
-                                          : static_cast<const int*>(r.idx)[t * r.top + k];
-                if (e >= 0 && e < r.experts)
-                    atomicAdd(&s.counts[e], 1);
-            }
-            valid += sub == 0 ? 1 : 0;
-        } else {
+    while (walk.left_of_warp > 0) {
+        const int at = walk.at, left = walk.left;
+        float x[U][NC][VEC], top[U], sum[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < NC; ++i)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
-                    x[i][v] = -INFINITY;
+                    x[u][i][v] = element<T, VEC>(raw[u][i], v);
+        walk.next();
+        load();  // the next rows, on their way while these are worked on
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            top[u] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    top[u] = fmaxf(top[u], x[u][i][v]);
         }
-        softmax_row<VEC, NC>(x, W);
+        group_max<U>(top, W);
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
+        for (int u = 0; u < U; ++u) {
+            top[u] = top[u] == -INFINITY ? 0.f : top[u];
+            exponentials<NC, VEC>(x[u], top[u]);
+            sum[u] = 0.f;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                acc[i][v] += x[i][v];
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    sum[u] += x[u][i][v];
+        }
+        group_sum<U>(sum, W);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float inv = sum[u] == 0.f ? 0.f : __fdividef(1.f, sum[u]);
+            if (sub == 0 && u * per_warp < left)
+                rows[at + u * per_warp] = make_float2(top[u], inv);
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    acc[i][v] = fmaf(x[u][i][v], inv, acc[i][v]);
+        }
     }
     // groups of a warp that hold the same columns, then the warps of the CTA
 #pragma unroll
@@ -254,10 +405,10 @@ __device__ __forceinline__ void weights(const Router& r, const Result& out, cons
 
 // dlogits of the rows of CTA `cta` of `ctas`
 template <class T, class D, int VEC, int NC>
-__device__ __forceinline__ void cta_grads(const Router& r, const Result& out, int W, int cta, int ctas, const Smem& s) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int sub = lane & (W - 1), per_warp = 32 / W;
-    const T* logits = static_cast<const T*>(r.logits);
+__device__ __forceinline__ void cta_grads(const Router& r, const Result& out, int W, int cta, int ctas, const Smem& s,
+                                          const float2* rows) {
+    constexpr int U = rows_in_flight<VEC, NC>();
+    const int sub = threadIdx.x & (W - 1), per_warp = 32 / W;
     float w[NC][VEC];
 #pragma unroll
     for (int i = 0; i < NC; ++i)
@@ -266,59 +417,81 @@ __device__ __forceinline__ void cta_grads(const Router& r, const Result& out, in
             const int c = (i * W + sub) * VEC + v;
             w[i][v] = c < r.experts ? s.w[c] : 0.f;
         }
-    const int64_t step = static_cast<int64_t>(ctas) * kWarps * per_warp;
-    for (int64_t base = (static_cast<int64_t>(cta) * kWarps + warp) * per_warp; base < r.tokens; base += step) {
-        const int64_t t = base + lane / W;
-        const bool here = t < r.tokens, live = here && (r.mask == nullptr || r.mask[t] != 0);
-        float x[NC][VEC];
-        if (live) {
-            load_row<T, VEC, NC>(logits + t * r.ld, W, sub, r.experts, x);
-        } else {
+    Walk<T, VEC, NC> walk(r, W, cta, ctas);
+    uint32_t raw[U][NC][words_of<T, VEC>()];
+    float2 row[U];
+    bool here[U];
+    auto load = [&]() {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            here[u] = walk.live(u);
+            row[u] = here[u] ? rows[walk.at + u * per_warp] : make_float2(0.f, 0.f);
+            load_row<T, VEC, NC>(walk.row(u), here[u], W, sub, r.experts, raw[u]);
+        }
+    };
+    load();
+    while (walk.left_of_warp > 0) {
+        const int at = walk.at, left = walk.left;
+        float x[U][NC][VEC], inv[U], dot[U];
+        bool live[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            dot[u] = 0.f;
+            live[u] = here[u];
+            inv[u] = row[u].y;
 #pragma unroll
             for (int i = 0; i < NC; ++i)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
-                    x[i][v] = -INFINITY;
-        }
-        softmax_row<VEC, NC>(x, W);
-        float dot = 0.f;
+                    x[u][i][v] = element<T, VEC>(raw[u][i], v);
+            exponentials<NC, VEC>(x[u], row[u].x);
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                dot += x[i][v] * w[i][v];
-        for (int o = W >> 1; o > 0; o >>= 1)
-            dot += __shfl_xor_sync(0xffffffffu, dot, o);
-        if (!here || (out.accumulate && !live))
-            continue;
-        D* row = static_cast<D*>(out.dlogits) + t * out.ldd;
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int c = (i * W + sub) * VEC;
-            if (c >= r.experts)
-                continue;
-            float d[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                d[v] = x[i][v] * (w[i][v] - dot);
-            if (out.accumulate) {
-                float o[VEC];
-                load_vec<VEC>(row + c, o);
+            for (int i = 0; i < NC; ++i)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
-                    d[v] += o[v];
+                    dot[u] = fmaf(x[u][i][v], w[i][v], dot[u]);
+        }
+        walk.next();
+        load();
+        group_sum<U>(dot, W);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u * per_warp >= left || (out.accumulate && !live[u]))
+                continue;
+            D* to = static_cast<D*>(out.dlogits) + static_cast<int64_t>(at + u * per_warp) * out.ldd;
+            dot[u] *= inv[u];
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int c = (i * W + sub) * VEC;
+                if (c >= r.experts)
+                    continue;
+                float d[VEC];
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    d[v] = x[u][i][v] * inv[u] * (w[i][v] - dot[u]);
+                if (out.accumulate) {
+                    float o[VEC];
+                    load_old<VEC>(to + c, o);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v)
+                        d[v] += o[v];
+                }
+                store_vec<VEC>(to + c, d);
             }
-            store_vec<VEC>(row + c, d);
         }
     }
 }
 
+// (three CTAs on an SM where the registers of a row allow it)
 template <class T, int VEC, int NC>
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster) stats_kernel(const Router r, int W, char* partial) {
+__global__ void __launch_bounds__(kThreads, VEC * NC <= 8 ? 3 : 1) __cluster_dims__(kCluster)
+        stats_kernel(const Router r, int W, char* partial, float2* rows) {
     extern __shared__ __align__(16) char raw[];
-    const Smem s = carve(raw, r.experts);
+    const Smem s = carve(raw, r.experts, true);
     cg::cluster_group cluster = cg::this_cluster();
-    cta_stats<T, VEC, NC>(r, W, blockIdx.x, gridDim.x, s);
+    // the second kernel may be set up meanwhile; it waits for this one's end before it reads anything
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    cta_stats<T, VEC, NC>(r, W, blockIdx.x, gridDim.x, s, rows);
     cluster.sync();
     float* sums = reinterpret_cast<float*>(partial) + static_cast<size_t>(blockIdx.x / kCluster) * partial_words(r.experts);
     int* counts = reinterpret_cast<int*>(sums + r.experts);
@@ -342,33 +515,59 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster) stats_ker
 }
 
 template <class T, class D, int VEC, int NC>
-__global__ void __launch_bounds__(kThreads) grad_kernel(const Router r, int W, const char* partial, int n_partials, const Result out) {
+__global__ void __launch_bounds__(kThreads, VEC * NC <= 8 ? 3 : 1) __cluster_dims__(kCluster)
+        grad_kernel(const Router r, int W, const char* partial, int n_partials, const float2* rows, const Result out) {
     extern __shared__ __align__(16) char raw[];
-    const Smem s = carve(raw, r.experts);
+    const Smem s = carve(raw, r.experts, false);
+    cg::cluster_group cluster = cg::this_cluster();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const float* sums = reinterpret_cast<const float*>(partial);
     const int words = partial_words(r.experts);
-    int valid = 0;
-    for (int k = 0; k < n_partials; ++k)
-        valid += reinterpret_cast<const int*>(sums)[static_cast<size_t>(k) * words + 2 * r.experts];
-    weights(r, out, s, valid, blockIdx.x == 0, [&](int e, double& sum, int& count) {
-        sum = 0.0;
-        count = 0;
-        for (int k = 0; k < n_partials; ++k) {
-            const float* one = sums + static_cast<size_t>(k) * words;
-            sum += one[e];
-            count += reinterpret_cast<const int*>(one)[r.experts + e];
+    // this CTA's eighth of the experts, G lanes each on the partial sums
+    const int per = (r.experts + kCluster - 1) / kCluster;
+    int G = 32;
+    while (G * per > kThreads)
+        G >>= 1;
+    {
+        const int mine = threadIdx.x / G, e = cluster.block_rank() * per + mine;
+        double sum = 0.0;
+        int count = 0;
+        if (mine < per && e < r.experts)
+            for (int k = threadIdx.x % G; k < n_partials; k += G) {
+                const float* one = sums + static_cast<size_t>(k) * words;
+                sum += one[e];
+                count += reinterpret_cast<const int*>(one)[r.experts + e];
+            }
+        for (int o = G >> 1; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            count += __shfl_xor_sync(0xffffffffu, count, o);
         }
+        if (mine < per && e < r.experts && threadIdx.x % G == 0) {
+            s.total[e] = sum;
+            s.counts[e] = count;
+        }
+    }
+    int valid = 0;
+    for (int k = threadIdx.x & 31; k < n_partials; k += 32)
+        valid += reinterpret_cast<const int*>(sums)[static_cast<size_t>(k) * words + 2 * r.experts];
+    valid = __reduce_add_sync(0xffffffffu, valid);
+    cluster.sync();
+    weights(r, out, s, valid, blockIdx.x == 0, [&](int e, double& sum, int& count) {
+        sum = *cluster.map_shared_rank(s.total + e, e / per);
+        count = *cluster.map_shared_rank(s.counts + e, e / per);
     });
+    cluster.sync();
     if (out.dlogits != nullptr)
-        cta_grads<T, D, VEC, NC>(r, out, W, blockIdx.x, gridDim.x, s);
+        cta_grads<T, D, VEC, NC>(r, out, W, blockIdx.x, gridDim.x, s, rows);
 }
 
 template <class T, class D, int VEC, int NC>
-__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster) small_kernel(const Router r, int W, const Result out) {
+__global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster)
+        small_kernel(const Router r, int W, float2* rows, const Result out) {
     extern __shared__ __align__(16) char raw[];
-    const Smem s = carve(raw, r.experts);
+    const Smem s = carve(raw, r.experts, true);
     cg::cluster_group cluster = cg::this_cluster();
-    cta_stats<T, VEC, NC>(r, W, blockIdx.x, gridDim.x, s);
+    cta_stats<T, VEC, NC>(r, W, blockIdx.x, gridDim.x, s, rows);  // (a CTA reads the rows that it wrote itself)
     cluster.sync();
     int valid = 0;
     for (int c = 0; c < kCluster; ++c)
@@ -383,22 +582,22 @@ __global__ void __launch_bounds__(kThreads) __cluster_dims__(kCluster) small_ker
     });
     cluster.sync();
     if (out.dlogits != nullptr)
-        cta_grads<T, D, VEC, NC>(r, out, W, blockIdx.x, gridDim.x, s);
+        cta_grads<T, D, VEC, NC>(r, out, W, blockIdx.x, gridDim.x, s, rows);
 }
 
-// How a row is laid over lanes: vectors of four where the rows' addresses allow it
+// How a row is laid over lanes: 16-byte vectors where the rows' addresses allow it, then 8 bytes of bf16
 struct Shape {
     int vec, W, nc;
 };
+bool vectors(const Router& r, const Result* out, int vec) {
+    bool ok = r.experts % vec == 0 && r.ld % vec == 0 && reinterpret_cast<uintptr_t>(r.logits) % (vec * (r.bf16 ? 2 : 4)) == 0;
+    if (out != nullptr && out->dlogits != nullptr)
+        ok = ok && out->ldd % vec == 0 && reinterpret_cast<uintptr_t>(out->dlogits) % (out->d_bf16 ? vec * 2 : 16) == 0;
+    return ok;
+}
 Shape shape(const Router& r, const Result* out) {
-    const uintptr_t size = r.bf16 ? 2 : 4;
-    bool four = r.experts % 4 == 0 && r.ld % 4 == 0 && reinterpret_cast<uintptr_t>(r.logits) % (4 * size) == 0;
-    if (out != nullptr && out->dlogits != nullptr) {
-        const uintptr_t d = out->d_bf16 ? 2 : 4;
-        four = four && out->ldd % 4 == 0 && reinterpret_cast<uintptr_t>(out->dlogits) % (4 * d) == 0;
-    }
     Shape s;
-    s.vec = four ? 4 : 1;
+    s.vec = r.bf16 && vectors(r, out, 8) ? 8 : vectors(r, out, 4) ? 4 : 1;
     const int units = (r.experts + s.vec - 1) / s.vec;
     s.W = 1;
     while (s.W < 32 && s.W < units)
@@ -421,53 +620,59 @@ bool bad(const Router& r, const Result& o) {
                                      reinterpret_cast<uintptr_t>(o.dlogits) % (o.d_bf16 ? 2 : 4) != 0));
 }
 
-// Calls go(kernel tag) with the types and the layout as template arguments
+// Calls go(vector, columns) with the layout as template arguments
 template <class T, class F>
 cudaError_t pick_row(const Shape& s, F go) {
-    if (s.vec == 4) {
-        switch (s.nc) {
-            case 1: return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-            case 2: return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
-            case 4: return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{});
-            default: return go(std::integral_constant<int, 4>{}, std::integral_constant<int, 8>{});
-        }
+#define MGK_ROW(V, N) \
+    if (s.vec == V && s.nc == N) \
+    return go(std::integral_constant<int, V>{}, std::integral_constant<int, N>{})
+    if constexpr (sizeof(T) == 2) {
+        MGK_ROW(8, 1);
+        MGK_ROW(8, 2);
+        MGK_ROW(8, 4);
     }
-    switch (s.nc) {
-        case 1: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 1>{});
-        case 2: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
-        case 4: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
-        case 8: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-        case 16: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-        default: return go(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
-    }
+    MGK_ROW(4, 1);
+    MGK_ROW(4, 2);
+    MGK_ROW(4, 4);
+    MGK_ROW(4, 8);
+    MGK_ROW(1, 1);
+    MGK_ROW(1, 2);
+    MGK_ROW(1, 4);
+    MGK_ROW(1, 8);
+    MGK_ROW(1, 16);
+    MGK_ROW(1, 32);
+#undef MGK_ROW
+    return cudaErrorInvalidValue;
 }
 
-// CTAs for `tokens` rows: at most two rounds of four resident CTAs per SM
-int row_ctas(const Router& r, const Shape& s, int most) {
-    const int64_t per_cta = static_cast<int64_t>(kWarps) * (32 / s.W);
-    const int64_t need = (r.tokens + per_cta - 1) / per_cta;
-    return static_cast<int>(need < 1 ? 1 : need > most ? most : need);
+float2* rows_of(void* workspace, const Router& r) {
+    return reinterpret_cast<float2*>(static_cast<char*>(workspace) +
+                                     static_cast<size_t>(kMaxPartials) * partial_words(r.experts) * 4);
 }
 
 }  // namespace
 
+size_t workspace_bytes(int tokens, int experts) {
+    return static_cast<size_t>(kMaxPartials) * partial_words(experts) * 4 + static_cast<size_t>(tokens) * sizeof(float2);
+}
+
 int partials(int tokens, int experts) {
-    // as many clusters as there is work for: at least 32 KB of float32 logits a CTA
+    // as many clusters as there is work for: at least 16 KB of float32 logits a CTA, three CTAs an SM at most
     const int64_t elements = static_cast<int64_t>(tokens) * experts;
-    const int64_t want = elements / (8192 * kCluster);
+    const int64_t want = elements / (4096 * kCluster);
     return static_cast<int>(want < 1 ? 1 : want > kMaxPartials ? kMaxPartials : want);
 }
 
-cudaError_t launch_stats(const Router& r, void* partial, cudaStream_t stream) {
-    if (bad(r) || partial == nullptr || reinterpret_cast<uintptr_t>(partial) % 16 != 0)
+cudaError_t launch_stats(const Router& r, void* workspace, cudaStream_t stream) {
+    if (bad(r) || workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return cudaErrorInvalidValue;
     const Shape s = shape(r, nullptr);
     const int grid = partials(r.tokens, r.experts) * kCluster;
     auto typed = [&](auto t) {
         using T = decltype(t);
         return pick_row<T>(s, [&](auto vec, auto nc) {
-            stats_kernel<T, decltype(vec)::value, decltype(nc)::value>
-                    <<<grid, kThreads, smem_bytes(r.experts), stream>>>(r, s.W, static_cast<char*>(partial));
+            stats_kernel<T, decltype(vec)::value, decltype(nc)::value><<<grid, kThreads, smem_bytes(r.experts, true), stream>>>(
+                    r, s.W, static_cast<char*>(workspace), rows_of(workspace, r));
             count_launch();
             return cudaGetLastError();
         });
@@ -475,20 +680,34 @@ cudaError_t launch_stats(const Router& r, void* partial, cudaStream_t stream) {
     return r.bf16 ? typed(__nv_bfloat16{}) : typed(float{});
 }
 
-cudaError_t launch_grad(const Router& r, const void* partial, int n_partials, const Result& out, cudaStream_t stream) {
+cudaError_t launch_grad(const Router& r, const void* partial, int n_partials, const void* workspace, const Result& out,
+                        bool follows_stats, cudaStream_t stream) {
     if (bad(r) || bad(r, out) || partial == nullptr || reinterpret_cast<uintptr_t>(partial) % 16 != 0 || n_partials < 1 ||
-        n_partials > kMaxPartials)
+        n_partials > kMaxPartials || workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return cudaErrorInvalidValue;
     const Shape s = shape(r, &out);
-    const int grid = row_ctas(r, s, 148 * 8);
     auto typed = [&](auto t, auto d) {
         using T = decltype(t);
         using D = decltype(d);
         return pick_row<T>(s, [&](auto vec, auto nc) {
-            grad_kernel<T, D, decltype(vec)::value, decltype(nc)::value><<<grid, kThreads, smem_bytes(r.experts), stream>>>(
-                    r, s.W, static_cast<const char*>(partial), n_partials, out);
+            constexpr int V = decltype(vec)::value, N = decltype(nc)::value;
+            const int64_t per_cta = static_cast<int64_t>(kWarps) * (32 / s.W) * rows_in_flight<V, N>();
+            int64_t clusters = (r.tokens + per_cta * kCluster - 1) / (per_cta * kCluster);
+            clusters = clusters < 1 ? 1 : clusters > kMaxPartials ? kMaxPartials : clusters;
+            cudaLaunchAttribute attr{};
+            attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr.val.programmaticStreamSerializationAllowed = 1;
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = static_cast<unsigned>(clusters * kCluster);
+            cfg.blockDim = kThreads;
+            cfg.dynamicSmemBytes = smem_bytes(r.experts, false);
+            cfg.stream = stream;
+            cfg.attrs = &attr;
+            cfg.numAttrs = follows_stats ? 1 : 0;
+            const cudaError_t e = cudaLaunchKernelEx(&cfg, grad_kernel<T, D, V, N>, r, s.W, static_cast<const char*>(partial),
+                                                     n_partials, static_cast<const float2*>(rows_of(const_cast<void*>(workspace), r)), out);
             count_launch();
-            return cudaGetLastError();
+            return e;
         });
     };
     if (!r.bf16)
@@ -496,18 +715,19 @@ cudaError_t launch_grad(const Router& r, const void* partial, int n_partials, co
     return out.d_bf16 ? typed(__nv_bfloat16{}, __nv_bfloat16{}) : typed(__nv_bfloat16{}, float{});
 }
 
-cudaError_t launch_small(const Router& r, const Result& out, cudaStream_t stream) {
-    if (bad(r) || bad(r, out))
+bool is_small(int tokens, int experts) { return static_cast<int64_t>(tokens) * experts <= 65536; }
+
+cudaError_t launch_small(const Router& r, void* workspace, const Result& out, cudaStream_t stream) {
+    if (bad(r) || bad(r, out) || !is_small(r.tokens, r.experts) || workspace == nullptr ||
+        reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
         return cudaErrorInvalidValue;
-    if (static_cast<int64_t>(r.tokens) * r.experts > 65536)
-        return cudaErrorNotSupported;
     const Shape s = shape(r, &out);
     auto typed = [&](auto t, auto d) {
         using T = decltype(t);
         using D = decltype(d);
         return pick_row<T>(s, [&](auto vec, auto nc) {
             small_kernel<T, D, decltype(vec)::value, decltype(nc)::value>
-                    <<<kCluster, kThreads, smem_bytes(r.experts), stream>>>(r, s.W, out);
+                    <<<kCluster, kThreads, smem_bytes(r.experts, true), stream>>>(r, s.W, rows_of(workspace, r), out);
             count_launch();
             return cudaGetLastError();
         });

@@ -9,7 +9,7 @@ namespace balance {
 
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxTop = 64;
-constexpr int kMaxPartials = 64;
+constexpr int kMaxPartials = 48;
 
 // float [E] sums of probabilities, then int32 [E] pairs per expert, then int32 tokens that count, padded to 4
 __host__ __device__ constexpr int partial_words(int experts) { return (2 * experts + 1 + 3) / 4 * 4; }
@@ -24,9 +24,11 @@ struct Router {
     int tokens, experts, top;
 };
 
+// The workspace holds kMaxPartials such records and two float32 a token (a row's maximum and reciprocal sum).
+size_t workspace_bytes(int tokens, int experts);
 // Number of partial sums that launch_stats writes for this size (1 .. kMaxPartials).
 int partials(int tokens, int experts);
-cudaError_t launch_stats(const Router& r, void* partial, cudaStream_t stream);
+cudaError_t launch_stats(const Router& r, void* workspace, cudaStream_t stream);
 
 struct Result {
     float coef;
@@ -37,10 +39,13 @@ struct Result {
     int64_t ldd;
     bool accumulate;
 };
-// `n_partials` partial sums as launch_stats wrote them (one, if they were added up over ranks meanwhile).
-cudaError_t launch_grad(const Router& r, const void* partial, int n_partials, const Result& out, cudaStream_t stream);
-// Both for a problem that one cluster handles in a single launch; cudaErrorNotSupported when it is larger.
-cudaError_t launch_small(const Router& r, const Result& out, cudaStream_t stream);
+// `n_partials` partial sums as launch_stats wrote them (one, if they were added up over ranks meanwhile) and the
+// workspace that it wrote for the same router.  `follows_stats`: launch_stats is the stream's last launch.
+cudaError_t launch_grad(const Router& r, const void* partial, int n_partials, const void* workspace, const Result& out,
+                        bool follows_stats, cudaStream_t stream);
+// Both in a single launch for a problem that one cluster handles.
+bool is_small(int tokens, int experts);
+cudaError_t launch_small(const Router& r, void* workspace, const Result& out, cudaStream_t stream);
 
 }  // namespace balance
 }  // namespace mgk

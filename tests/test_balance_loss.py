@@ -228,10 +228,12 @@ def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
         r = _lib.Router(**{**ok, **bad})
         assert lib.megray_balance(r, out, 64, None) in (6, -1), bad
         assert lib.megray_balance_stats(r, 64, None) in (6, -1), bad
-        assert lib.megray_balance_grad(r, 64, 1, out, None) in (6, -1), bad
+        assert lib.megray_balance_grad(r, 64, 1, 64, out, None) in (6, -1), bad
     r = _lib.Router(**ok)
     assert lib.megray_balance_stats(r, None, None) == -1 and lib.megray_balance_stats(r, 72, None) == -1
-    for n in (0, 65):
-        assert lib.megray_balance_grad(r, 64, n, out, None) == -1
+    for n in (0, 49):
+        assert lib.megray_balance_grad(r, 64, n, 64, out, None) == -1
+    assert lib.megray_balance_grad(r, None, 1, 64, out, None) == -1 and lib.megray_balance_grad(r, 64, 1, None, out, None) == -1
+    assert lib.megray_balance(r, out, None, None) == -1 and lib.megray_balance(r, out, 72, None) == -1
     for bad in ((None, 64, 64, 8, 7), (64, None, 64, 8, 7), (64, 64, 66, 8, 7), (64, 64, 64, 7, 7), (64, 64, 64, 8, 10)):
         assert lib.megray_balance(r, _lib.BalanceOut(*bad, 0, 1.0), 64, None) == -1, bad
