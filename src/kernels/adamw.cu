@@ -31,6 +31,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "f32x2.cuh"
 #include "launch_count.h"
 
 namespace mgk {
@@ -140,28 +141,11 @@ __device__ __forceinline__ bool vector_ok(const T* p) {
     return (reinterpret_cast<uintptr_t>(p) & (4 * sizeof(T) - 1)) == 0;
 }
 
-// Two float32 products in one instruction, each rounded on its own
-struct Pair {
-    float x, y;
-};
-__device__ __forceinline__ Pair mul(Pair a, Pair b) {
-    Pair d;
-    asm("{\n .reg .b64 p, q, r;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n mul.rn.f32x2 r, p, q;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-// (one by one: a paired sum of paired products was contracted into fused multiply-adds)
-__device__ __forceinline__ Pair add(Pair a, Pair b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("{\n .reg .b64 p, q, r, s;\n mov.b64 p, {%2, %3};\n mov.b64 q, {%4, %5};\n mov.b64 r, {%6, %7};\n"
-        " fma.rn.f32x2 s, p, q, r;\n mov.b64 {%0, %1}, s;\n}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ Pair both(float x) { return {x, x}; }
+using f32x2::both;
+using f32x2::fma;
+using f32x2::mul;
+using f32x2::Pair;
+__device__ __forceinline__ Pair add_apart(Pair a, Pair b) { return {__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)}; }
 
 // four e4m3 numbers times a scale
 __device__ __forceinline__ void decode4(uint32_t code, float scale, float* f) {
@@ -182,12 +166,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-// the larger magnitude of a and those of b and c; a NaN is kept
-__device__ __forceinline__ float top_of(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
     return d;
 }
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -224,7 +202,7 @@ __device__ __forceinline__ float encode8(const float (&f)[8], uint32_t (&code)[2
     float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; i += 2)
-        t = top_of(t, f[i], f[i + 1]);
+        t = f32x2::max3_nan(t, fabsf(f[i]), fabsf(f[i + 1]));
     const float top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(t)));
     const float inv = top < kLeast ? 0.f : __fmul_rn(__frcp_rn(top), kTop);
 #pragma unroll
@@ -342,8 +320,8 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? 4 : 3) adamw_kernel(cons
             if (BITS == 8)
                 vv = mul(vv, vv);
             const Pair x = mul({g[i], g[i + 1]}, gs);
-            mm = add(mul(mm, b1), mul(x, c1));
-            vv = add(mul(vv, b2), mul(mul(x, x), c2));
+            mm = add_apart(mul(mm, b1), mul(x, c1));
+            vv = add_apart(mul(vv, b2), mul(mul(x, x), c2));
             m[i] = mm.x;
             m[i + 1] = mm.y;
             v[i] = vv.x;

@@ -24,6 +24,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "f32x2.cuh"
 #include "gemm_device.cuh"
 #include "launch_count.h"
 
@@ -83,14 +84,35 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
             : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 384 threads start with 168 registers each; the eight warps that hold rows of scores take 224, the other four
-// keep 56: 256 x 224 + 128 x 56 = 384 x 168
-__device__ __forceinline__ void registers_of_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
-__device__ __forceinline__ void registers_of_others() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+// 384 threads start with 168 registers each; the eight warps that hold rows of scores take 216, the other four
+// keep 72: 256 x 216 + 128 x 72 = 384 x 168
+__device__ __forceinline__ void registers_of_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
+__device__ __forceinline__ void registers_of_others() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+using f32x2::both;
+using f32x2::max3_nan;
+using f32x2::Pair;
+
+// 2^x for x <= 8 without the special-function unit: x = n + f with n the nearest whole number (it is left in the low
+// bits of x + 1.5 2^23) and |f| <= 1/2, a polynomial of degree 4 for 2^f that is 1 at 0 (the least largest relative
+// error, found by linear programming: 2.9e-6 in float32, a 700th of half a bf16 step), n added to its exponent.
+// At 2^-127 and below the result is zero, exactly: masked scores are -infinity.
+__device__ __forceinline__ Pair ex2_poly(Pair x) {
+    const float magic = 12582912.f;
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
+    const Pair t = f32x2::add(x, both(magic)), f = f32x2::add(x, f32x2::fma(t, both(-1.f), both(magic)));
+    Pair p = f32x2::fma(both(0.009582852944731712f), f, both(0.055906426161527634f));
+    p = f32x2::fma(p, f, both(0.24024099111557007f));
+    p = f32x2::fma(p, f, both(0.6931241750717163f));
+    p = f32x2::fma(p, f, both(1.f));
+    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
+    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
+    return p;
 }
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -241,6 +263,7 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint
 // stays below 2^8, which changes nothing in its relative precision, and the rescaling is rare.
 constexpr int FWD_THREADS = 384;
 constexpr int FWD_STAGES = 4;
+constexpr int FWD_POLY = 1, FWD_POLY_OF = 4;  // of so many pairs of exponentials, so many by polynomial
 
 template <int DP>
 constexpr int tile_bytes() { return DP / 64 * CHUNK_BYTES; }
@@ -258,8 +281,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring + FWD_STAGES * TB);
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * FWD_STAGES;
     const uint32_t q_full = empty0 + 8 * FWD_STAGES;          // one per tile
-    const uint32_t s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 16, side = o_full + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FWD_STAGES + 9);
+    const uint32_t s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 32, side = o_full + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FWD_STAGES + 11);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -278,7 +301,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         for (int t = 0; t < 2; ++t) {
             mbar_init(q_full + 8 * t, 1);
             mbar_init(s_full + 8 * t, 1);
-            mbar_init(p_ready + 8 * t, 4);
+            mbar_init(p_ready + 16 * t, 4);  // the halves of a tile's probabilities
+            mbar_init(p_ready + 16 * t + 8, 4);
             mbar_init(o_full + 8 * t, 1);
         }
         mbar_init(side, 1);
@@ -367,13 +391,18 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                 for (int t = 0; ok && t < 2; ++t) {
                     if (j >= n_blocks[t])
                         continue;
-                    ok = mbar_wait(p_ready + 8 * t, j & 1, wc);
+                    for (int h = 0; ok && h < 2; ++h) {
+                        ok = mbar_wait(p_ready + 16 * t + 8 * h, j & 1, wc);
+                        if (!ok)
+                            break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            umma_ts(t_o + t * TILE, t_s + t * TILE + 8 * (4 * h + kk), desc_mn(v, 4 * h + kk), id_o,
+                                    j != 0 || h != 0 || kk != 0);
+                    }
                     if (!ok)
                         break;
-                    tc_fence_after();
-#pragma unroll
-                    for (int kk = 0; kk < TILE / 16; ++kk)
-                        umma_ts(t_o + t * TILE, t_s + t * TILE + 8 * kk, desc_mn(v, kk), id_o, j != 0 || kk != 0);
                     if (j + 1 == n_blocks[t]) {
                         umma_commit_cg1(o_full + 8 * t);
                     } else {
@@ -426,16 +455,18 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 32; e += 2)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    top[i] = fmaxf(top[i], __uint_as_float(s[i][e]));
-            const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    top[i] = max3_nan(top[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
+            const float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
+            // each row goes by its own maximum (also where a score is NaN: the row becomes NaN)
+            const bool rises = !((mx - m) * c <= 8.f) && row < w.len;
             if (j == 0) {
                 m = mx;
-            } else if (__any_sync(0xffffffffu, (mx - m) * c > 8.f)) {
+            } else if (__any_sync(0xffffffffu, rises)) {
                 // the product that last added to O has retired: the scores' barrier came after it
-                const float to = fmaxf(m, mx), f = ex2((m - to) * c);
+                const float to = rises ? max3_nan(m, mx, mx) : m, f = ex2((m - to) * c);
                 m = to;
                 l *= f;
                 for (int d = 0; d < p.dim; d += 32) {
@@ -448,27 +479,32 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                     tmem_st_x32(o_at + d, o);
                 }
             }
-            const float mc = m * c;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const Pair cc = both(c), mc = both(-m * c);
+            Pair sum[2] = {both(0.f), both(0.f)};
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
+            for (int h = 0; h < 2; ++h) {
                 uint32_t pk[32];
 #pragma unroll
-                for (int e = 0; e < 64; e += 2) {
-                    const float a = ex2(fmaf(__uint_as_float(s[i + e / 32][e % 32]), c, -mc));
-                    const float b = ex2(fmaf(__uint_as_float(s[i + e / 32][e % 32 + 1]), c, -mc));
-                    sum[(e >> 1) & 1] += a;
-                    sum[2 + ((e >> 1) & 1)] += b;
-                    pk[e / 2] = pack2<FP16>(a, b);
+                for (int e = 0; e < 32; ++e) {
+                    const uint32_t* at = &s[2 * h + e / 16][2 * (e % 16)];
+                    Pair x = f32x2::fma({__uint_as_float(at[0]), __uint_as_float(at[1])}, cc, mc);
+                    if (e % FWD_POLY_OF < FWD_POLY) {
+                        x = ex2_poly(x);
+                    } else {
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                    }
+                    sum[e & 1] = f32x2::add(sum[e & 1], x);
+                    pk[e] = pack2<FP16>(x.x, x.y);
                 }
-                tmem_st_x32(s_at + 16 * i, pk);
+                tmem_st_x32(s_at + 32 * h, pk);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0)
+                    mbar_arrive(p_ready + 16 * t + 8 * h);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(p_ready + 8 * t);
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         if (ok && n_blocks[t] > 0 && __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, 0, wc))) {
             tc_fence_after();
