@@ -38,6 +38,7 @@ using namespace mgk::ptx;
 constexpr int TILE = 128;
 constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 elements
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int POLY = 1, POLY_OF = 4;  // of so many pairs of exponentials, so many by polynomial
 constexpr uint64_t WAIT_NS = 4000000000ull;
 
 struct Params {
@@ -99,20 +100,26 @@ using f32x2::Pair;
 
 // 2^x for x <= 8 without the special-function unit: x = n + f with n the nearest whole number (it is left in the low
 // bits of x + 1.5 2^23) and |f| <= 1/2, a polynomial of degree 4 for 2^f that is 1 at 0 (the least largest relative
-// error, found by linear programming: 2.9e-6 in float32, a 700th of half a bf16 step), n added to its exponent.
-// At 2^-127 and below the result is zero, exactly: masked scores are -infinity.
+// error, found by linear programming: 2.9e-6 in float32, a 700th of half a bf16 step), times 2^n.  At 2^-127 and
+// below the result is zero, exactly: masked scores are -infinity.  A NaN stays one.
 __device__ __forceinline__ Pair ex2_poly(Pair x) {
     const float magic = 12582912.f;
-    x.x = fmaxf(x.x, -127.f);
-    x.y = fmaxf(x.y, -127.f);
+    x.x = max3_nan(x.x, -127.f, -127.f);
+    x.y = max3_nan(x.y, -127.f, -127.f);
     const Pair t = f32x2::add(x, both(magic)), f = f32x2::add(x, f32x2::fma(t, both(-1.f), both(magic)));
     Pair p = f32x2::fma(both(0.009582852944731712f), f, both(0.055906426161527634f));
     p = f32x2::fma(p, f, both(0.24024099111557007f));
     p = f32x2::fma(p, f, both(0.6931241750717163f));
     p = f32x2::fma(p, f, both(1.f));
-    p.x = __uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23));
-    p.y = __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23));
-    return p;
+    return f32x2::mul(p, {__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                          __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)});
+}
+// 2^x of a pair by one way or the other
+template <bool POLY>
+__device__ __forceinline__ Pair ex2_pair(Pair x) {
+    if (POLY)
+        return ex2_poly(x);
+    return {ex2(x.x), ex2(x.y)};
 }
 template <bool FP16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -233,6 +240,16 @@ __device__ __forceinline__ uint8_t* align_1024(uint8_t* p) {
     return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~static_cast<uintptr_t>(1023));
 }
 
+// Swizzled tiles start at multiples of 1024 bytes.  Dynamic shared memory does, and the backward kernels have no room
+// for shifting it: if it ever does not, the error flag is set and nothing is done.
+__device__ __forceinline__ bool unaligned(const uint8_t* smem, const Params& p) {
+    if ((smem_u32(smem) & 1023) == 0)
+        return false;
+    if (threadIdx.x == 0 && p.error_flag != nullptr)
+        *p.error_flag = 1;
+    return true;
+}
+
 // Writes one row of `dim` float32 TMEM columns times `f`, rounded, to global memory
 template <bool FP16>
 __device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint16_t* to, bool write) {
@@ -263,7 +280,6 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint
 // stays below 2^8, which changes nothing in its relative precision, and the rescaling is rare.
 constexpr int FWD_THREADS = 384;
 constexpr int FWD_STAGES = 4;
-constexpr int FWD_POLY = 1, FWD_POLY_OF = 4;  // of so many pairs of exponentials, so many by polynomial
 
 template <int DP>
 constexpr int tile_bytes() { return DP / 64 * CHUNK_BYTES; }
@@ -488,12 +504,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                 for (int e = 0; e < 32; ++e) {
                     const uint32_t* at = &s[2 * h + e / 16][2 * (e % 16)];
                     Pair x = f32x2::fma({__uint_as_float(at[0]), __uint_as_float(at[1])}, cc, mc);
-                    if (e % FWD_POLY_OF < FWD_POLY) {
-                        x = ex2_poly(x);
-                    } else {
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
-                    }
+                    x = e % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
                     sum[e & 1] = f32x2::add(sum[e & 1], x);
                     pk[e] = pack2<FP16>(x.x, x.y);
                 }
@@ -558,10 +569,13 @@ __global__ void __launch_bounds__(256) delta_kernel(const uint16_t* __restrict__
 //   tensor cores:  S(j+1)         dQ += dS(j) K, dP(j+1) = dO V^T      S(j+2) ...
 //   warpgroups:    dS(j) from dP  P(j+1) from S                        dS(j+1) ...
 constexpr int BWD_THREADS = 384;  // 8 warps of arithmetic, MMA, TMA, row statistics (dK/dV only), one idle
-constexpr int BWD_STAGES = 2;
+// Ring slots: the operand that both the scores and the last product of an iteration read (K, or Q) is held for one
+// and a half iterations and needs three for the next to arrive in time, the other two.  (Two each: the tensor cores
+// waited 1400 of 4600 cycles an iteration for Q.)
+constexpr int LONG_STAGES = 3, SHORT_STAGES = 2;
 
 template <int DP>
-constexpr int bwd_smem() { return (2 + 2 * BWD_STAGES) * tile_bytes<DP>() + BWD_STAGES * 2 * TILE * 4 + 1024 + 512; }
+constexpr int bwd_smem() { return (2 + LONG_STAGES + SHORT_STAGES) * tile_bytes<DP>() + SHORT_STAGES * 2 * TILE * 4 + 256; }
 
 // Half a row (64 columns) of P: TMEM column `s_at` on
 template <class F>
@@ -583,14 +597,16 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     constexpr int TB = tile_bytes<DP>();
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = align_1024(smem_raw);  // Q, dO, then K slots, then V slots
-    uint8_t *ring_k = smem + 2 * TB, *ring_v = ring_k + BWD_STAGES * TB;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(ring_v + BWD_STAGES * TB + BWD_STAGES * 2 * TILE * 4);
-    const uint32_t k_full = smem_u32(bars), k_empty = k_full + 16, v_full = k_empty + 16, v_empty = v_full + 16;
-    const uint32_t q_full = v_empty + 16, s_full = q_full + 8, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8,
+    extern __shared__ __align__(1024) uint8_t smem[];  // Q, dO, then K slots, then V slots
+    if (unaligned(smem, p))
+        return;
+    uint8_t *ring_k = smem + 2 * TB, *ring_v = ring_k + LONG_STAGES * TB;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(ring_v + SHORT_STAGES * TB);
+    const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8 * LONG_STAGES, v_full = k_empty + 8 * LONG_STAGES,
+                   v_empty = v_full + 8 * SHORT_STAGES;
+    const uint32_t q_full = v_empty + 8 * SHORT_STAGES, s_full = q_full + 8, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8,
                    done = ds_ready + 8, side = done + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (LONG_STAGES + SHORT_STAGES) + 7);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -604,7 +620,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     }
     if (warp == 9 && lane == 0) {
         *abort_flag = 0;
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
             mbar_init(k_full + 8 * s, 1);
         mbar_init(q_full, 2);
         mbar_init(s_full, 1);
@@ -644,13 +660,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         __syncwarp();
         uint32_t side_phase = 0;
         for (int j = 0; j < n; ++j) {
-            const int s = j % BWD_STAGES, live = w.len - j * TILE;
-            const uint32_t ph = ((j / BWD_STAGES) & 1) ^ 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * s, ph, wc)) ||
+            const int s = j % LONG_STAGES, sv = j % SHORT_STAGES, live = w.len - j * TILE;
+            if (!__all_sync(0xffffffffu, mbar_wait(k_empty + 8 * s, ((j / LONG_STAGES) & 1) ^ 1, wc)) ||
                 !feed<DP>(ring_k + s * TB, &map_k, k_full + 8 * s, side, side_phase, kv_head, w.start + j * TILE, live, wc))
                 break;
-            if (!__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * s, ph, wc)) ||
-                !feed<DP>(ring_v + s * TB, &map_v, v_full + 8 * s, side, side_phase, kv_head, w.start + j * TILE, live, wc))
+            if (!__all_sync(0xffffffffu, mbar_wait(v_empty + 8 * sv, ((j / SHORT_STAGES) & 1) ^ 1, wc)) ||
+                !feed<DP>(ring_v + sv * TB, &map_v, v_full + 8 * sv, side, side_phase, kv_head, w.start + j * TILE, live, wc))
                 break;
         }
     } else if (warp == 8) {
@@ -660,8 +675,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
             const uint32_t q = smem_u32(smem), d_o = q + TB;
             auto scores = [&](int j) {
-                const int s = j % BWD_STAGES;
-                if (!mbar_wait(k_full + 8 * s, (j / BWD_STAGES) & 1, wc))
+                const int s = j % LONG_STAGES;
+                if (!mbar_wait(k_full + 8 * s, (j / LONG_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
                 for (int kk = 0; kk < ksteps; ++kk)
@@ -670,8 +685,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 return true;
             };
             auto grads = [&](int j) {
-                const int s = j % BWD_STAGES;
-                if (!mbar_wait(v_full + 8 * s, (j / BWD_STAGES) & 1, wc))
+                const int s = j % SHORT_STAGES;
+                if (!mbar_wait(v_full + 8 * s, (j / SHORT_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
                 for (int kk = 0; kk < ksteps; ++kk)
@@ -688,11 +703,11 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 if (!ok)
                     break;
                 tc_fence_after();
-                const uint32_t k = smem_u32(ring_k) + j % BWD_STAGES * TB;
+                const uint32_t k = smem_u32(ring_k) + j % LONG_STAGES * TB;
 #pragma unroll
                 for (int kk = 0; kk < TILE / 16; ++kk)
                     umma_ts(t_dq, a_half(t_dp, kk), desc_mn(k, kk), id_d, j != 0 || kk != 0);
-                umma_commit_cg1(k_empty + 8 * (j % BWD_STAGES));
+                umma_commit_cg1(k_empty + 8 * (j % LONG_STAGES));
                 if (j + 1 < n)
                     ok = grads(j + 1);
             }
@@ -724,8 +739,12 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             if (lane == 0)
                 mbar_arrive(s_free);
 #pragma unroll
-            for (int e = 0; e < 64; ++e)
-                pr[e] = ex2(fmaf(pr[e], c, -lse2));
+            for (int e = 0; e < 64; e += 2) {
+                Pair x = f32x2::fma({pr[e], pr[e + 1]}, both(c), both(-lse2));
+                x = e / 2 % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
+                pr[e] = x.x;
+                pr[e + 1] = x.y;
+            }
             if (j * TILE + TILE > w.len || (p.causal && j * TILE + TILE > r0)) {
 #pragma unroll
                 for (int e = 0; e < 64; ++e)
@@ -777,16 +796,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     constexpr int TB = tile_bytes<DP>();
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = align_1024(smem_raw);  // K, V, then Q slots, then dO slots, then lse and delta of the slots' rows
-    uint8_t *ring_q = smem + 2 * TB, *ring_do = ring_q + BWD_STAGES * TB;
-    float* stats = reinterpret_cast<float*>(ring_do + BWD_STAGES * TB);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(stats + BWD_STAGES * 2 * TILE);
-    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 16, o_full = q_empty + 16, o_empty = o_full + 16;
-    const uint32_t st_full = o_empty + 16, st_empty = st_full + 16;
-    const uint32_t kv_full = st_empty + 16, s_full = kv_full + 8, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
+    // K, V, then Q slots, then dO slots, then -lse log2 e and delta of the rows of two blocks
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (unaligned(smem, p))
+        return;
+    uint8_t *ring_q = smem + 2 * TB, *ring_do = ring_q + LONG_STAGES * TB;
+    float* stats = reinterpret_cast<float*>(ring_do + SHORT_STAGES * TB);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(stats + SHORT_STAGES * 2 * TILE);
+    const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * LONG_STAGES, o_full = q_empty + 8 * LONG_STAGES,
+                   o_empty = o_full + 8 * SHORT_STAGES;
+    const uint32_t st_full = o_empty + 8 * SHORT_STAGES, st_empty = st_full + 8 * SHORT_STAGES;
+    const uint32_t kv_full = st_empty + 8 * SHORT_STAGES, s_full = kv_full + 8, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
                    done = ds_ready + 8, side = done + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * LONG_STAGES + 4 * SHORT_STAGES + 7);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -801,9 +823,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     }
     if (warp == 9 && lane == 0) {
         *abort_flag = 0;
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
             mbar_init(q_full + 8 * s, 1);
-        for (int s = 0; s < BWD_STAGES; ++s) {
+        for (int s = 0; s < SHORT_STAGES; ++s) {
             mbar_init(st_full + 8 * s, 1);
             mbar_init(st_empty + 8 * s, 8);
         }
@@ -845,27 +867,27 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         __syncwarp();
         uint32_t side_phase = 0;
         for (int it = 0; it < n; ++it) {
-            const int s = it % BWD_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
-            const uint32_t ph = ((it / BWD_STAGES) & 1) ^ 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(q_empty + 8 * s, ph, wc)) ||
+            const int s = it % LONG_STAGES, so = it % SHORT_STAGES, head = kv_head * group + it / per_head;
+            const int q0 = (i0 + it % per_head) * TILE;
+            if (!__all_sync(0xffffffffu, mbar_wait(q_empty + 8 * s, ((it / LONG_STAGES) & 1) ^ 1, wc)) ||
                 !feed<DP>(ring_q + s * TB, &map_q, q_full + 8 * s, side, side_phase, head, w.start + q0, w.len - q0, wc))
                 break;
-            if (!__all_sync(0xffffffffu, mbar_wait(o_empty + 8 * s, ph, wc)) ||
-                !feed<DP>(ring_do + s * TB, &map_do, o_full + 8 * s, side, side_phase, head, w.start + q0, w.len - q0, wc))
+            if (!__all_sync(0xffffffffu, mbar_wait(o_empty + 8 * so, ((it / SHORT_STAGES) & 1) ^ 1, wc)) ||
+                !feed<DP>(ring_do + so * TB, &map_do, o_full + 8 * so, side, side_phase, head, w.start + q0, w.len - q0, wc))
                 break;
         }
     } else if (warp == 10) {
         registers_of_others();
-        // lse (times log2 e) and delta of every block's rows; a row behind the end has probabilities of zero
+        // -lse log2 e and delta of every block's rows; a row behind the end has probabilities of zero
         for (int it = 0; it < n; ++it) {
-            const int s = it % BWD_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
-            if (!__all_sync(0xffffffffu, mbar_wait(st_empty + 8 * s, ((it / BWD_STAGES) & 1) ^ 1, wc)))
+            const int s = it % SHORT_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
+            if (!__all_sync(0xffffffffu, mbar_wait(st_empty + 8 * s, ((it / SHORT_STAGES) & 1) ^ 1, wc)))
                 break;
             float* to = stats + s * 2 * TILE;
             const int64_t at = static_cast<int64_t>(head) * p.tokens + w.start + q0;
             for (int r = lane; r < TILE; r += 32) {
                 const bool live = q0 + r < w.len;
-                to[r] = live ? p.lse[at + r] * LOG2E : INFINITY;
+                to[r] = live ? p.lse[at + r] * -LOG2E : -INFINITY;
                 to[TILE + r] = live ? p.delta[at + r] : 0.f;
             }
             __syncwarp();
@@ -879,8 +901,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
             const uint32_t k = smem_u32(smem), v = k + TB;
             auto scores = [&](int it) {
-                const int s = it % BWD_STAGES;
-                if (!mbar_wait(q_full + 8 * s, (it / BWD_STAGES) & 1, wc))
+                const int s = it % LONG_STAGES;
+                if (!mbar_wait(q_full + 8 * s, (it / LONG_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
                 for (int kk = 0; kk < ksteps; ++kk)
@@ -889,8 +911,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 return true;
             };
             auto grads = [&](int it) {
-                const int s = it % BWD_STAGES;
-                if (!mbar_wait(o_full + 8 * s, (it / BWD_STAGES) & 1, wc))
+                const int s = it % SHORT_STAGES;
+                if (!mbar_wait(o_full + 8 * s, (it / SHORT_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
                 for (int kk = 0; kk < ksteps; ++kk)
@@ -900,15 +922,15 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             };
             bool ok = mbar_wait(kv_full, 0, wc) && scores(0) && grads(0);
             for (int it = 0; ok && it < n; ++it) {
-                const int s = it % BWD_STAGES;
+                const int s = it % LONG_STAGES, so = it % SHORT_STAGES;
                 ok = mbar_wait(p_ready, it & 1, wc);
                 if (!ok)
                     break;
                 tc_fence_after();
 #pragma unroll
                 for (int kk = 0; kk < TILE / 16; ++kk)
-                    umma_ts(t_dv, a_half(t_s, kk), desc_mn(smem_u32(ring_do) + s * TB, kk), id_d, it != 0 || kk != 0);
-                umma_commit_cg1(o_empty + 8 * s);
+                    umma_ts(t_dv, a_half(t_s, kk), desc_mn(smem_u32(ring_do) + so * TB, kk), id_d, it != 0 || kk != 0);
+                umma_commit_cg1(o_empty + 8 * so);
                 if (it + 1 < n)
                     ok = scores(it + 1);
                 ok = ok && mbar_wait(ds_ready, it & 1, wc);
@@ -934,22 +956,26 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         const float c = p.scale * LOG2E;
         bool ok = true;
         for (int it = 0; it < n; ++it) {
-            const int s = it % BWD_STAGES, q0 = (i0 + it % per_head) * TILE + half * 64;
-            const float4* lse2 = reinterpret_cast<const float4*>(stats + s * 2 * TILE + half * 64);
-            const float4* delta = lse2 + TILE / 4;
+            const int s = it % SHORT_STAGES, q0 = (i0 + it % per_head) * TILE + half * 64;
+            const float4* minus_lse = reinterpret_cast<const float4*>(stats + s * 2 * TILE + half * 64);
+            const float4* delta = minus_lse + TILE / 4;
             float pr[64];
-            ok = __all_sync(0xffffffffu, mbar_wait(st_full + 8 * s, (it / BWD_STAGES) & 1, wc) && mbar_wait(s_full, it & 1, wc));
+            ok = __all_sync(0xffffffffu, mbar_wait(st_full + 8 * s, (it / SHORT_STAGES) & 1, wc) && mbar_wait(s_full, it & 1, wc));
             if (!ok)
                 break;
             tc_fence_after();
             half_row(t_s + half * 64 + lanes, [&](int e, float x) { pr[e] = x; });
 #pragma unroll
             for (int e = 0; e < 64; e += 4) {
-                const float4 z = lse2[e / 4];
-                pr[e] = ex2(fmaf(pr[e], c, -z.x));
-                pr[e + 1] = ex2(fmaf(pr[e + 1], c, -z.y));
-                pr[e + 2] = ex2(fmaf(pr[e + 2], c, -z.z));
-                pr[e + 3] = ex2(fmaf(pr[e + 3], c, -z.w));
+                const float4 z = minus_lse[e / 4];
+                Pair a = f32x2::fma({pr[e], pr[e + 1]}, both(c), {z.x, z.y});
+                Pair b = f32x2::fma({pr[e + 2], pr[e + 3]}, both(c), {z.z, z.w});
+                a = e / 2 % POLY_OF < POLY ? ex2_pair<true>(a) : ex2_pair<false>(a);
+                b = (e / 2 + 1) % POLY_OF < POLY ? ex2_pair<true>(b) : ex2_pair<false>(b);
+                pr[e] = a.x;
+                pr[e + 1] = a.y;
+                pr[e + 2] = b.x;
+                pr[e + 3] = b.y;
             }
             if (p.causal && it % per_head == 0) {
 #pragma unroll
