@@ -4,8 +4,9 @@
 //   delta = rowsum(O * dO)     dV = P^T dO        dS = P * (dO V^T - delta)
 //   dQ = scale dS K            dK = scale dS^T Q  (dK and dV summed over the query heads of a group)
 //
-// Three kernels of one shape: a TMA warp, a warp whose elected lane issues every tcgen05.mma, and two warpgroups
-// that turn scores into probabilities, one thread a row (a TMEM lane).  Tiles are 128 rows of 64 (dim <= 64) or
+// Three kernels of one shape: a TMA warp, a warp whose elected lane issues every tcgen05.mma, and sixteen warps
+// that turn scores into probabilities.  (Sixteen and not eight with twice the columns each: a warp alone on its
+// scheduler waits for its own exponentials two cycles of three.)  Tiles are 128 rows of 64 (dim <= 64) or
 // 128 elements in 128-byte-swizzled shared memory; a dimension in between is filled up with zeros by TMA, and the
 // products run over the multiple of 16 that covers it.  P and dS are the products' left operands straight from
 // TMEM: they are written over the scores they come from, as 16-bit pairs, and never pass through shared memory.
@@ -62,15 +63,33 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* map, uint3
             "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
             : "memory");
 }
-// D (+)= A B with A in TMEM: lane = row, a 32-bit column holds two neighbours along K
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Products of one CTA with 128 rows.  Operands in shared memory are given by the low word of their descriptor; the
+// high one (8-row groups 1024 bytes apart, 128-byte swizzle) is the same for all.  A in TMEM: lane = row, a 32-bit
+// column holds two neighbours along K.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
     asm volatile(
             "{\n"
             " .reg .pred p;\n"
+            " .reg .b64 da, db;\n"
+            " mov.b64 da, {%1, %5};\n"
+            " mov.b64 db, {%2, %5};\n"
             " setp.ne.b32 p, %4, 0;\n"
-            " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n"
             "}\n" ::"r"(d),
-            "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+            "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(DESC_HI)
+            : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+    asm volatile(
+            "{\n"
+            " .reg .pred p;\n"
+            " .reg .b64 db;\n"
+            " mov.b64 db, {%2, %5};\n"
+            " setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n"
+            "}\n" ::"r"(d),
+            "r"(a), "r"(b), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(DESC_HI)
             : "memory");
 }
 __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -84,11 +103,21 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
             "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
             : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+            "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+            "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+            "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+            "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+            : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// 384 threads start with 168 registers each; the eight warps that hold rows of scores take 216, the other four
-// keep 72: 256 x 216 + 128 x 72 = 384 x 168
-__device__ __forceinline__ void registers_of_rows() { asm volatile("setmaxnreg.inc.sync.aligned.u32 216;"); }
-__device__ __forceinline__ void registers_of_others() { asm volatile("setmaxnreg.dec.sync.aligned.u32 72;"); }
+// Moves registers from warps that need few to those that hold scores; the sums may not pass what the threads of the
+// block started with
+template <int N>
+__device__ __forceinline__ void set_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void set_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -143,13 +172,39 @@ __device__ __forceinline__ uint32_t idesc_for(int n, bool b_mn) {
     return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |
            (static_cast<uint32_t>(TILE >> 4) << 24);
 }
-// Tile [128 rows, dim] as an operand whose K axis is dim: step kk of 16 elements
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int kk) {
-    return umma_smem_desc_sw128(tile + (kk >> 2) * CHUNK_BYTES + (kk & 3) * 32, 16, 1024);
+// Tile [128 rows, dim] as an operand whose K axis is dim, or whose K axis is the rows: low word of the descriptor,
+// and what a step of 16 elements or rows adds to it
+__device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return ((tile & 0x3FFFF) >> 4) | (1u << 16); }
+__device__ __forceinline__ constexpr uint32_t step_k(int kk) { return ((kk >> 2) * CHUNK_BYTES + (kk & 3) * 32) >> 4; }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) {
+    return ((tile & 0x3FFFF) >> 4) | (static_cast<uint32_t>(CHUNK_BYTES >> 4) << 16);
 }
-// The same tile as an operand whose K axis is the rows: step kk of 16 rows
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int kk) {
-    return umma_smem_desc_sw128(tile + kk * 2048, CHUNK_BYTES, 1024);
+__device__ __forceinline__ constexpr uint32_t step_mn(int kk) { return kk * 2048 >> 4; }
+
+// The two kinds of products.  Everything an instruction needs is an addition away: the one thread that issues them
+// was what the kernels waited for when each built its descriptors (75 cycles an instruction that takes 64).
+// [128, 128] (+)= tile tile^T over `ksteps` x 16 elements of the dimension
+template <int DP>
+__device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int ksteps) {
+#pragma unroll
+    for (int kk = 0; kk < DP / 16; ++kk)
+        if (kk < ksteps)
+            umma_ss(d, a + step_k(kk), b + step_k(kk), idesc, kk != 0);
+}
+// [128, dim] (+)= P tile over the tile's 128 rows; WIDTH scores (32, 64 or 128) of a row were written by one thread,
+// where they were
+template <int WIDTH>
+__device__ __forceinline__ void multiply_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+    for (int kk = 0; kk < TILE / 16; ++kk)
+        umma_ts(d, a + kk / (WIDTH / 16) * WIDTH + kk % (WIDTH / 16) * 8, b + step_mn(kk), idesc, kk != 0 || accumulate);
+}
+// A wait of the thread that issues products: it polls a while before it sleeps, which wakes it sooner
+__device__ __forceinline__ bool issue_wait(uint32_t bar, uint32_t parity, const WaitCtx& w) {
+    for (int i = 0; i < 256; ++i)
+        if (mbar_test_wait(bar, parity))
+            return true;
+    return mbar_wait(bar, parity, w);
 }
 
 // ---------------------------------------------------------------- which sequence a tile belongs to
@@ -250,10 +305,11 @@ __device__ __forceinline__ bool unaligned(const uint8_t* smem, const Params& p) 
     return true;
 }
 
-// Writes one row of `dim` float32 TMEM columns times `f`, rounded, to global memory
+// Writes columns [from, to) of one row of float32 TMEM columns times `f`, rounded, to global memory; `from` is a
+// multiple of 32
 template <bool FP16>
-__device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint16_t* to, bool write) {
-    for (int c = 0; c < dim; c += 32) {
+__device__ __forceinline__ void store_row(uint32_t taddr, int from, int to, float f, uint16_t* row, bool write) {
+    for (int c = from; c < to; c += 32) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(taddr + c, r);
         tmem_ld_wait(r);
@@ -261,12 +317,12 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint
             continue;
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
-            if (c + i < dim) {
+            if (c + i < to) {
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     w[k] = pack2<FP16>(__uint_as_float(r[i + 2 * k]) * f, __uint_as_float(r[i + 2 * k + 1]) * f);
-                *reinterpret_cast<uint4*>(to + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(row + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
             }
         }
     }
@@ -278,7 +334,8 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int dim, float f, uint
 // scores of its tile, the tensor cores work for the other tile.  The running maximum only moves when the
 // new one is more than 2^8 larger (then the accumulator is rescaled in TMEM by the threads that own its rows): P
 // stays below 2^8, which changes nothing in its relative precision, and the rescaling is rare.
-constexpr int FWD_THREADS = 384;
+constexpr int FWD_ROW_WARPS = 8, FWD_MMA = 8, FWD_TMA = 9;  // (and two warps that idle)
+constexpr int FWD_THREADS = 32 * (FWD_ROW_WARPS + 4);
 constexpr int FWD_STAGES = 4;
 
 template <int DP>
@@ -297,8 +354,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring + FWD_STAGES * TB);
     const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * FWD_STAGES;
     const uint32_t q_full = empty0 + 8 * FWD_STAGES;          // one per tile
-    const uint32_t s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 32, side = o_full + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FWD_STAGES + 11);
+    const uint32_t s_full = q_full + 16, p_ready = s_full + 16, o_full = p_ready + 16, side = o_full + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * FWD_STAGES + 9);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -310,15 +367,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         if (lane == 0)
             *where = w;
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == FWD_TMA && lane == 0) {
         *abort_flag = 0;
         for (int s = 0; s < 2 * FWD_STAGES; ++s)
             mbar_init(full0 + 8 * s, 1);
         for (int t = 0; t < 2; ++t) {
             mbar_init(q_full + 8 * t, 1);
             mbar_init(s_full + 8 * t, 1);
-            mbar_init(p_ready + 16 * t, 4);  // the halves of a tile's probabilities
-            mbar_init(p_ready + 16 * t + 8, 4);
+            mbar_init(p_ready + 8 * t, FWD_ROW_WARPS / 2);
             mbar_init(o_full + 8 * t, 1);
         }
         mbar_init(side, 1);
@@ -332,7 +388,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const Where w = *where;
     if (w.len == 0)
         return;  // all threads alike, before anything is allocated
-    if (warp == 8) {
+    if (warp == FWD_MMA) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
@@ -354,8 +410,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const int n = max(n_blocks[0], n_blocks[1]);
     WaitCtx wc{abort_flag, WAIT_NS};
 
-    if (warp == 9) {
-        registers_of_others();
+    if (warp == FWD_TMA) {
+        set_registers_down<72>();  // 256 x 216 + 128 x 72 = 384 x 168
         const int kv_head = head / (p.heads / p.kv_heads);
         if (elect_one()) {
             load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
@@ -375,71 +431,79 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                           live, wc))
                 break;
         }
-    } else if (warp == 8) {
-        registers_of_others();
+    } else if (warp == FWD_MMA) {
+        set_registers_down<72>();  // 256 x 216 + 128 x 72 = 384 x 168
         if (elect_one()) {
             const int ksteps = (p.dim + 15) / 16;
             const uint32_t id_s = idesc_for<FP16>(TILE, false), id_o = idesc_for<FP16>(ksteps * 16, true);
-            auto scores = [&](int t, int it) {
-                const uint32_t q = smem_u32(smem) + t * TB, k = smem_u32(ring) + it % FWD_STAGES * TB;
-                for (int kk = 0; kk < ksteps; ++kk)
-                    umma_f16_cg1(t_s + t * TILE, desc_k(q, kk), desc_k(k, kk), id_s, kk != 0);
+            const uint32_t q_desc = desc_k(smem_u32(smem)), ring0 = smem_u32(ring);
+            auto scores = [&](int t, uint32_t k) {
+                multiply_rows<DP>(t_s + t * TILE, q_desc + t * (TB >> 4), k, id_s, ksteps);
                 umma_commit_cg1(s_full + 8 * t);
             };
-            auto loaded = [&](int it) { return mbar_wait(full0 + 8 * (it % FWD_STAGES), (it / FWD_STAGES) & 1, wc); };
-            bool ok = mbar_wait(q_full, 0, wc) && loaded(0);
+            bool ok = issue_wait(q_full, 0, wc) && issue_wait(full0, 0, wc);
             if (ok) {
                 tc_fence_after();
-                scores(0, 0);
+                scores(0, desc_k(ring0));
                 if (n_blocks[1] > 0) {
-                    ok = mbar_wait(q_full + 8, 0, wc);
+                    ok = issue_wait(q_full + 8, 0, wc);
                     if (ok)
-                        scores(1, 0);
+                        scores(1, desc_k(ring0));
                 }
                 if (n > 2)  // the slot is used again
                     umma_commit_cg1(empty0);
             }
+            int sv = 1, sk = 2;       // slots of this block's values and of the next one's keys
+            uint32_t pv = 0, pk = 0;  // and the parities of their barriers
+            bool v_here = false, k_here = false;
             for (int j = 0; ok && j < n; ++j) {
-                const int iv = 2 * j + 1, ik = 2 * j + 2;
-                ok = loaded(iv);
-                const uint32_t v = smem_u32(ring) + iv % FWD_STAGES * TB;
+                const uint32_t v = desc_mn(ring0 + sv * TB), k = desc_k(ring0 + sk * TB);
                 bool next = false;
-                for (int t = 0; ok && t < 2; ++t) {
-                    if (j >= n_blocks[t])
-                        continue;
-                    for (int h = 0; ok && h < 2; ++h) {
-                        ok = mbar_wait(p_ready + 16 * t + 8 * h, j & 1, wc);
-                        if (!ok)
-                            break;
-                        tc_fence_after();
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            umma_ts(t_o + t * TILE, t_s + t * TILE + 8 * (4 * h + kk), desc_mn(v, 4 * h + kk), id_o,
-                                    j != 0 || h != 0 || kk != 0);
-                    }
+                for (int t = 0; t < 2; ++t) {
+                    if (!ok || j >= n_blocks[t])
+                        continue;
+                    ok = (v_here || issue_wait(full0 + 8 * sv, pv, wc)) && issue_wait(p_ready + 8 * t, j & 1, wc);
                     if (!ok)
-                        break;
-                    if (j + 1 == n_blocks[t]) {
+                        continue;
+                    v_here = true;
+                    tc_fence_after();
+                    const bool last = j + 1 == n_blocks[t];
+                    if (!last && !k_here)  // (asked for early: its answer comes while the products are issued)
+                        k_here = mbar_test_wait(full0 + 8 * sk, pk);
+                    multiply_scores<TILE>(t_o + t * TILE, t_s + t * TILE, v, id_o, j != 0);
+                    if (last) {
                         umma_commit_cg1(o_full + 8 * t);
                     } else {
-                        if (!next)
-                            ok = loaded(ik);
+                        ok = k_here || issue_wait(full0 + 8 * sk, pk, wc);
+                        k_here = true;
                         next = true;
                         if (ok) {
                             tc_fence_after();
-                            scores(t, ik);  // over P of this block: products of one thread run in order
+                            scores(t, k);  // over P of this block: products of one thread run in order
                         }
                     }
                 }
                 if (next) {  // (behind the last block nobody waits for a free slot)
-                    umma_commit_cg1(empty0 + 8 * (iv % FWD_STAGES));
-                    umma_commit_cg1(empty0 + 8 * (ik % FWD_STAGES));
+                    umma_commit_cg1(empty0 + 8 * sv);
+                    umma_commit_cg1(empty0 + 8 * sk);
+                }
+                v_here = k_here = false;
+                sv += 2;
+                if (sv >= FWD_STAGES) {
+                    sv -= FWD_STAGES;
+                    pv ^= 1;
+                }
+                sk += 2;
+                if (sk >= FWD_STAGES) {
+                    sk -= FWD_STAGES;
+                    pk ^= 1;
                 }
             }
         }
         __syncwarp();
-    } else if (warp < 8) {
-        registers_of_rows();
+    } else if (warp < FWD_ROW_WARPS) {
+        set_registers_up<216>();
         const int t = warp >> 2;
         const int row = (threadIdx.x & 127) + r0 + t * TILE;  // in the sequence
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -509,29 +573,29 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                     pk[e] = pack2<FP16>(x.x, x.y);
                 }
                 tmem_st_x32(s_at + 32 * h, pk);
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0)
-                    mbar_arrive(p_ready + 16 * t + 8 * h);
             }
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(p_ready + 8 * t);
         }
         if (ok && n_blocks[t] > 0 && __all_sync(0xffffffffu, mbar_wait(o_full + 8 * t, 0, wc))) {
             tc_fence_after();
             const bool write = row < w.len;
             const int64_t at = w.start + row;
-            store_row<FP16>(o_at, p.dim, 1.f / l, p.out0 + at * p.row0 + head * p.head0, write);
+            store_row<FP16>(o_at, 0, p.dim, 1.f / l, p.out0 + at * p.row0 + head * p.head0, write);
             if (write)
                 p.lse[static_cast<int64_t>(head) * p.tokens + at] = m * p.scale + logf(l);
         }
     } else {
-        registers_of_others();
+        set_registers_down<72>();  // 256 x 216 + 128 x 72 = 384 x 168
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8)
+    if (warp == FWD_MMA)
         tmem_dealloc_cg1(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
         *p.error_flag = 1;
@@ -565,10 +629,12 @@ __global__ void __launch_bounds__(256) delta_kernel(const uint16_t* __restrict__
 
 // ================================================================ backward: dQ
 //
-// A CTA takes 128 queries of one head.  Both warpgroups work on every tile of scores, a thread on half a row.
+// A CTA takes 128 queries of one head.  All row warps work on every tile of scores, a thread on a quarter of a row.
 //   tensor cores:  S(j+1)         dQ += dS(j) K, dP(j+1) = dO V^T      S(j+2) ...
-//   warpgroups:    dS(j) from dP  P(j+1) from S                        dS(j+1) ...
-constexpr int BWD_THREADS = 384;  // 8 warps of arithmetic, MMA, TMA, row statistics (dK/dV only), one idle
+//   row warps:     dS(j) from dP  P(j+1) from S                        dS(j+1) ...
+constexpr int ROW_WARPS = 16, MMA_WARP = 16, TMA_WARP = 17, STAT_WARP = 18;  // (and a warp that idles)
+constexpr int BWD_THREADS = 32 * (ROW_WARPS + 4);  // 512 x 104 + 128 x 64 = 640 x 96 registers
+
 // Ring slots: the operand that both the scores and the last product of an iteration read (K, or Q) is held for one
 // and a half iterations and needs three for the next to arrive in time, the other two.  (Two each: the tensor cores
 // waited 1400 of 4600 cycles an iteration for Q.)
@@ -577,20 +643,15 @@ constexpr int LONG_STAGES = 3, SHORT_STAGES = 2;
 template <int DP>
 constexpr int bwd_smem() { return (2 + LONG_STAGES + SHORT_STAGES) * tile_bytes<DP>() + SHORT_STAGES * 2 * TILE * 4 + 256; }
 
-// Half a row (64 columns) of P: TMEM column `s_at` on
-template <class F>
-__device__ __forceinline__ void half_row(uint32_t s_at, F each) {
-    uint32_t s[2][32];
-    tmem_ld_32x32b_x32(s_at, s[0]);
-    tmem_ld_32x32b_x32(s_at + 32, s[1]);
-    tmem_ld_wait(s[0]);
-    tmem_ld_wait(s[1]);
+// A quarter of a row (32 columns)
+__device__ __forceinline__ void load_quarter(uint32_t at, float (&x)[32]) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(at, r);
+    tmem_ld_wait(r);
 #pragma unroll
-    for (int e = 0; e < 64; ++e)
-        each(e, __uint_as_float(s[e / 32][e % 32]));
+    for (int e = 0; e < 32; ++e)
+        x[e] = __uint_as_float(r[e]);
 }
-// A operand of step kk of 16: the two halves of a row were written where their scores were
-__device__ __forceinline__ uint32_t a_half(uint32_t t, int kk) { return t + (kk < 4 ? 8 * kk : 64 + 8 * (kk - 4)); }
 
 template <int DP, bool FP16>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
@@ -618,15 +679,15 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if (lane == 0)
             *where = w;
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == TMA_WARP && lane == 0) {
         *abort_flag = 0;
         for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
             mbar_init(k_full + 8 * s, 1);
         mbar_init(q_full, 2);
         mbar_init(s_full, 1);
-        mbar_init(s_free, 8);
+        mbar_init(s_free, ROW_WARPS);
         mbar_init(dp_full, 1);
-        mbar_init(ds_ready, 8);
+        mbar_init(ds_ready, ROW_WARPS);
         mbar_init(done, 1);
         mbar_init(side, 1);
         mbar_fence_init();
@@ -636,7 +697,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const Where w = *where;
     if (w.len == 0)
         return;
-    if (warp == 8) {
+    if (warp == MMA_WARP) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
@@ -650,8 +711,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const int n = (keys + TILE - 1) / TILE;
     WaitCtx wc{abort_flag, WAIT_NS};
 
-    if (warp == 9) {
-        registers_of_others();
+    if (warp == TMA_WARP) {
+        set_registers_down<64>();
         const int kv_head = head / (p.heads / p.kv_heads);
         if (elect_one()) {
             load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
@@ -668,56 +729,54 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 !feed<DP>(ring_v + sv * TB, &map_v, v_full + 8 * sv, side, side_phase, kv_head, w.start + j * TILE, live, wc))
                 break;
         }
-    } else if (warp == 8) {
-        registers_of_others();
+    } else if (warp == MMA_WARP) {
+        set_registers_down<64>();
         if (elect_one()) {
             const int ksteps = (p.dim + 15) / 16;
             const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
-            const uint32_t q = smem_u32(smem), d_o = q + TB;
-            auto scores = [&](int j) {
+            const uint32_t q = desc_k(smem_u32(smem)), d_o = q + (TB >> 4), k0 = smem_u32(ring_k), v0 = smem_u32(ring_v);
+            auto scores = [&](int j, bool here) {
                 const int s = j % LONG_STAGES;
-                if (!mbar_wait(k_full + 8 * s, (j / LONG_STAGES) & 1, wc))
+                if (!here && !issue_wait(k_full + 8 * s, (j / LONG_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
-                for (int kk = 0; kk < ksteps; ++kk)
-                    umma_f16_cg1(t_s, desc_k(q, kk), desc_k(smem_u32(ring_k) + s * TB, kk), id_s, kk != 0);
+                multiply_rows<DP>(t_s, q, desc_k(k0 + s * TB), id_s, ksteps);
                 umma_commit_cg1(s_full);
                 return true;
             };
-            auto grads = [&](int j) {
+            auto grads = [&](int j, bool here) {
                 const int s = j % SHORT_STAGES;
-                if (!mbar_wait(v_full + 8 * s, (j / SHORT_STAGES) & 1, wc))
+                if (!here && !issue_wait(v_full + 8 * s, (j / SHORT_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
-                for (int kk = 0; kk < ksteps; ++kk)
-                    umma_f16_cg1(t_dp, desc_k(d_o, kk), desc_k(smem_u32(ring_v) + s * TB, kk), id_s, kk != 0);
+                multiply_rows<DP>(t_dp, d_o, desc_k(v0 + s * TB), id_s, ksteps);
                 umma_commit_cg1(dp_full);
                 umma_commit_cg1(v_empty + 8 * s);
                 return true;
             };
-            bool ok = mbar_wait(q_full, 0, wc) && scores(0) && grads(0);
+            bool ok = issue_wait(q_full, 0, wc) && scores(0, false) && grads(0, false);
             for (int j = 0; ok && j < n; ++j) {
-                if (j + 1 < n)
-                    ok = mbar_wait(s_free, j & 1, wc) && scores(j + 1);
-                ok = ok && mbar_wait(ds_ready, j & 1, wc);
+                if (j + 1 < n) {
+                    const bool here = mbar_test_wait(k_full + 8 * ((j + 1) % LONG_STAGES), ((j + 1) / LONG_STAGES) & 1);
+                    ok = issue_wait(s_free, j & 1, wc) && scores(j + 1, here);
+                }
+                ok = ok && issue_wait(ds_ready, j & 1, wc);
                 if (!ok)
                     break;
                 tc_fence_after();
-                const uint32_t k = smem_u32(ring_k) + j % LONG_STAGES * TB;
-#pragma unroll
-                for (int kk = 0; kk < TILE / 16; ++kk)
-                    umma_ts(t_dq, a_half(t_dp, kk), desc_mn(k, kk), id_d, j != 0 || kk != 0);
+                const bool here = j + 1 < n && mbar_test_wait(v_full + 8 * ((j + 1) % SHORT_STAGES), ((j + 1) / SHORT_STAGES) & 1);
+                multiply_scores<32>(t_dq, t_dp, desc_mn(k0 + j % LONG_STAGES * TB), id_d, j != 0);
                 umma_commit_cg1(k_empty + 8 * (j % LONG_STAGES));
                 if (j + 1 < n)
-                    ok = grads(j + 1);
+                    ok = grads(j + 1, here);
             }
             if (ok)
                 umma_commit_cg1(done);
         }
         __syncwarp();
-    } else if (warp < 8) {
-        registers_of_rows();
-        const int half = warp >> 2;
+    } else if (warp < ROW_WARPS) {
+        set_registers_up<104>();
+        const int part = warp >> 2;  // 32 columns of every tile
         const int row = (threadIdx.x & 127) + r0;
         const bool live = row < w.len;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -727,19 +786,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         const float lse2 = live ? p.lse[at] * LOG2E : 0.f, delta = live ? p.delta[at] : 0.f;
         bool ok = true;
         for (int j = 0; j < n; ++j) {
-            const int k0 = j * TILE + half * 64;
-            float pr[64];
+            const int k0 = j * TILE + part * 32;
+            float pr[32], dp[32];
             ok = __all_sync(0xffffffffu, mbar_wait(s_full, j & 1, wc));
             if (!ok)
                 break;
             tc_fence_after();
-            half_row(t_s + half * 64 + lanes, [&](int e, float s) { pr[e] = s; });
+            load_quarter(t_s + part * 32 + lanes, pr);
             tc_fence_before();
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(s_free);
 #pragma unroll
-            for (int e = 0; e < 64; e += 2) {
+            for (int e = 0; e < 32; e += 2) {
                 Pair x = f32x2::fma({pr[e], pr[e + 1]}, both(c), both(-lse2));
                 x = e / 2 % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
                 pr[e] = x.x;
@@ -747,7 +806,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             }
             if (j * TILE + TILE > w.len || (p.causal && j * TILE + TILE > r0)) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
+                for (int e = 0; e < 32; ++e)
                     if (k0 + e >= limit)
                         pr[e] = 0.f;
             }
@@ -755,13 +814,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             if (!ok)
                 break;
             tc_fence_after();
-            uint32_t pk[32];
-            half_row(t_dp + half * 64 + lanes, [&](int e, float dp) {
-                pr[e] *= dp - delta;
-                if (e & 1)
-                    pk[e / 2] = pack2<FP16>(pr[e - 1], pr[e]);
-            });
-            tmem_st_x32(t_dp + half * 64 + lanes, pk);
+            load_quarter(t_dp + part * 32 + lanes, dp);
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+                const Pair x = f32x2::mul({pr[e], pr[e + 1]}, f32x2::add({dp[e], dp[e + 1]}, both(-delta)));
+                pk[e / 2] = pack2<FP16>(x.x, x.y);
+            }
+            tmem_st_x16(t_dp + part * 32 + lanes, pk);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -770,16 +830,16 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         }
         if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, wc))) {
             tc_fence_after();
-            if (half == 0)
-                store_row<FP16>(t_dq + lanes, p.dim, p.scale, p.out0 + (w.start + static_cast<int64_t>(row)) * p.row0 + head * p.head0, live);
+            store_row<FP16>(t_dq + lanes, part * 32, min(p.dim, part * 32 + 32), p.scale,
+                            p.out0 + (w.start + static_cast<int64_t>(row)) * p.row0 + head * p.head0, live);
         }
     } else {
-        registers_of_others();
+        set_registers_down<64>();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8)
+    if (warp == MMA_WARP)
         tmem_dealloc_cg1(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
         *p.error_flag = 1;
@@ -789,14 +849,17 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 //
 // A CTA takes 128 keys of one key / value head and walks over the queries of every head of its group; rows of the
 // score tiles are keys, so P^T and dS^T are left operands as they stand.
-//   tensor cores:  dV += P^T(i) dO, S^T(i+1)    dK += dS^T(i) Q, dP^T(i+1)
-//   warpgroups:    dS(i) from dP                P(i+1) from S
+// Scores and their gradients take turns in one region of TMEM, A; probabilities and score gradients as 16-bit operands
+// lie in another, B, so that neither waits for the product that reads the other:
+//   tensor cores:  dV += P^T(i-1) dO, A = dP^T(i), dK += dS^T(i-1) Q, A = S^T(i+1), ...
+//   row warps:     P(i) from S(i) (in registers: A is free at once)    dS(i) from dP(i)
+// (P written over S and dS over dP, so that S(i+1) waited for dV: 3180 cycles an iteration; the products take 2048.)
 template <int DP, bool FP16>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
         dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                    const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     constexpr int TB = tile_bytes<DP>();
-    // K, V, then Q slots, then dO slots, then -lse log2 e and delta of the rows of two blocks
+    // K, V, then Q slots, then dO slots, then -lse log2 e and -delta of the rows of two blocks
     extern __shared__ __align__(1024) uint8_t smem[];
     if (unaligned(smem, p))
         return;
@@ -806,9 +869,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const uint32_t q_full = smem_u32(bars), q_empty = q_full + 8 * LONG_STAGES, o_full = q_empty + 8 * LONG_STAGES,
                    o_empty = o_full + 8 * SHORT_STAGES;
     const uint32_t st_full = o_empty + 8 * SHORT_STAGES, st_empty = st_full + 8 * SHORT_STAGES;
-    const uint32_t kv_full = st_empty + 8 * SHORT_STAGES, s_full = kv_full + 8, p_ready = s_full + 8, dp_full = p_ready + 8, ds_ready = dp_full + 8,
-                   done = ds_ready + 8, side = done + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * LONG_STAGES + 4 * SHORT_STAGES + 7);
+    const uint32_t kv_full = st_empty + 8 * SHORT_STAGES, s_full = kv_full + 8, s_free = s_full + 8, dp_full = s_free + 8,
+                   dp_free = dp_full + 8, ds_ready = dp_free + 8, dk_done = ds_ready + 8,
+                   done = dk_done + 8, side = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * LONG_STAGES + 4 * SHORT_STAGES + 9);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -821,19 +885,21 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if (lane == 0)
             *where = w;
     }
-    if (warp == 9 && lane == 0) {
+    if (warp == TMA_WARP && lane == 0) {
         *abort_flag = 0;
         for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
             mbar_init(q_full + 8 * s, 1);
         for (int s = 0; s < SHORT_STAGES; ++s) {
             mbar_init(st_full + 8 * s, 1);
-            mbar_init(st_empty + 8 * s, 8);
+            mbar_init(st_empty + 8 * s, ROW_WARPS);
         }
         mbar_init(kv_full, 2);
         mbar_init(s_full, 1);
-        mbar_init(p_ready, 8);
+        mbar_init(s_free, ROW_WARPS);
         mbar_init(dp_full, 1);
-        mbar_init(ds_ready, 8);
+        mbar_init(dp_free, ROW_WARPS);
+        mbar_init(ds_ready, ROW_WARPS);
+        mbar_init(dk_done, 1);
         mbar_init(done, 1);
         mbar_init(side, 1);
         mbar_fence_init();
@@ -843,7 +909,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const Where w = *where;
     if (w.len == 0)
         return;
-    if (warp == 8) {
+    if (warp == MMA_WARP) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
@@ -851,15 +917,15 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dv = tmem + 2 * TILE, t_dk = tmem + 3 * TILE;
+    const uint32_t t_a = tmem, t_p = tmem + TILE, t_ds = t_p + 64, t_dv = tmem + 2 * TILE, t_dk = tmem + 3 * TILE;
     const int k0 = w.local * TILE;               // the first keys, which the most queries see, come first
     const int i0 = p.causal ? w.local : 0;       // first block of queries that sees them
     const int per_head = w.tiles - i0;
     const int n = group * per_head;
     WaitCtx wc{abort_flag, WAIT_NS};
 
-    if (warp == 9) {
-        registers_of_others();
+    if (warp == TMA_WARP) {
+        set_registers_down<64>();
         if (elect_one()) {
             load_tile<DP>(smem_u32(smem), &map_k, kv_full, kv_head, w.start + k0);
             load_tile<DP>(smem_u32(smem) + TB, &map_v, kv_full, kv_head, w.start + k0);
@@ -876,9 +942,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 !feed<DP>(ring_do + so * TB, &map_do, o_full + 8 * so, side, side_phase, head, w.start + q0, w.len - q0, wc))
                 break;
         }
-    } else if (warp == 10) {
-        registers_of_others();
-        // -lse log2 e and delta of every block's rows; a row behind the end has probabilities of zero
+    } else if (warp == STAT_WARP) {
+        set_registers_down<64>();
+        // -lse log2 e and -delta of every block's rows; a row behind the end has probabilities of zero
         for (int it = 0; it < n; ++it) {
             const int s = it % SHORT_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
             if (!__all_sync(0xffffffffu, mbar_wait(st_empty + 8 * s, ((it / SHORT_STAGES) & 1) ^ 1, wc)))
@@ -888,85 +954,104 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             for (int r = lane; r < TILE; r += 32) {
                 const bool live = q0 + r < w.len;
                 to[r] = live ? p.lse[at + r] * -LOG2E : -INFINITY;
-                to[TILE + r] = live ? p.delta[at + r] : 0.f;
+                to[TILE + r] = live ? -p.delta[at + r] : 0.f;
             }
             __syncwarp();
             if (lane == 0)
                 mbar_arrive(st_full + 8 * s);
         }
-    } else if (warp == 8) {
-        registers_of_others();
+    } else if (warp == MMA_WARP) {
+        set_registers_down<64>();
         if (elect_one()) {
             const int ksteps = (p.dim + 15) / 16;
             const uint32_t id_s = idesc_for<FP16>(TILE, false), id_d = idesc_for<FP16>(ksteps * 16, true);
-            const uint32_t k = smem_u32(smem), v = k + TB;
-            auto scores = [&](int it) {
+            const uint32_t k = desc_k(smem_u32(smem)), v = k + (TB >> 4), rq = smem_u32(ring_q), ro = smem_u32(ring_do);
+            auto q_here = [&](int it) { return mbar_test_wait(q_full + 8 * (it % LONG_STAGES), (it / LONG_STAGES) & 1); };
+            auto o_here = [&](int it) { return mbar_test_wait(o_full + 8 * (it % SHORT_STAGES), (it / SHORT_STAGES) & 1); };
+            auto scores = [&](int it, bool here) {
                 const int s = it % LONG_STAGES;
-                if (!mbar_wait(q_full + 8 * s, (it / LONG_STAGES) & 1, wc))
+                if (!here && !issue_wait(q_full + 8 * s, (it / LONG_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
-                for (int kk = 0; kk < ksteps; ++kk)
-                    umma_f16_cg1(t_s, desc_k(k, kk), desc_k(smem_u32(ring_q) + s * TB, kk), id_s, kk != 0);
+                multiply_rows<DP>(t_a, k, desc_k(rq + s * TB), id_s, ksteps);
                 umma_commit_cg1(s_full);
                 return true;
             };
-            auto grads = [&](int it) {
+            auto grads = [&](int it, bool here) {
                 const int s = it % SHORT_STAGES;
-                if (!mbar_wait(o_full + 8 * s, (it / SHORT_STAGES) & 1, wc))
+                if (!here && !issue_wait(o_full + 8 * s, (it / SHORT_STAGES) & 1, wc))
                     return false;
                 tc_fence_after();
-                for (int kk = 0; kk < ksteps; ++kk)
-                    umma_f16_cg1(t_dp, desc_k(v, kk), desc_k(smem_u32(ring_do) + s * TB, kk), id_s, kk != 0);
+                multiply_rows<DP>(t_a, v, desc_k(ro + s * TB), id_s, ksteps);
                 umma_commit_cg1(dp_full);
                 return true;
             };
-            bool ok = mbar_wait(kv_full, 0, wc) && scores(0) && grads(0);
-            for (int it = 0; ok && it < n; ++it) {
-                const int s = it % LONG_STAGES, so = it % SHORT_STAGES;
-                ok = mbar_wait(p_ready, it & 1, wc);
-                if (!ok)
-                    break;
+            // (P is in place when dP has been read: both are told by one barrier)
+            auto add_dv = [&](int it) {
+                const int s = it % SHORT_STAGES;
+                multiply_scores<TILE>(t_dv, t_p, desc_mn(ro + s * TB), id_d, it != 0);
+                umma_commit_cg1(o_empty + 8 * s);
+            };
+            auto add_dk = [&](int it, bool here) {
+                const int s = it % LONG_STAGES;
+                if (!here && !issue_wait(ds_ready, it & 1, wc))
+                    return false;
                 tc_fence_after();
-#pragma unroll
-                for (int kk = 0; kk < TILE / 16; ++kk)
-                    umma_ts(t_dv, a_half(t_s, kk), desc_mn(smem_u32(ring_do) + so * TB, kk), id_d, it != 0 || kk != 0);
-                umma_commit_cg1(o_empty + 8 * so);
-                if (it + 1 < n)
-                    ok = scores(it + 1);
-                ok = ok && mbar_wait(ds_ready, it & 1, wc);
-                if (!ok)
-                    break;
-                tc_fence_after();
-#pragma unroll
-                for (int kk = 0; kk < TILE / 16; ++kk)
-                    umma_ts(t_dk, a_half(t_dp, kk), desc_mn(smem_u32(ring_q) + s * TB, kk), id_d, it != 0 || kk != 0);
+                multiply_scores<TILE>(t_dk, t_ds, desc_mn(rq + s * TB), id_d, it != 0);
                 umma_commit_cg1(q_empty + 8 * s);
-                if (it + 1 < n)
-                    ok = grads(it + 1);
+                umma_commit_cg1(dk_done);
+                return true;
+            };
+            // barriers are asked ahead of the products before which they are needed, so that the answers come while
+            // others are issued
+            bool ok = issue_wait(kv_full, 0, wc) && scores(0, false);
+            for (int it = 0; ok && it < n; ++it) {
+                const bool o_now = o_here(it);
+                if (it > 0)
+                    add_dv(it - 1);
+                ok = issue_wait(s_free, it & 1, wc);
+                if (!ok)
+                    break;
+                const bool ds_now = it > 0 && mbar_test_wait(ds_ready, (it - 1) & 1);
+                ok = grads(it, o_now);
+                const bool q_now = it + 1 < n && q_here(it + 1);
+                ok = ok && (it == 0 || add_dk(it - 1, ds_now)) && issue_wait(dp_free, it & 1, wc);
+                if (ok && it + 1 < n)
+                    ok = scores(it + 1, q_now);
+            }
+            if (ok) {
+                tc_fence_after();
+                add_dv(n - 1);
+                ok = add_dk(n - 1, false);
             }
             if (ok)
                 umma_commit_cg1(done);
         }
         __syncwarp();
-    } else if (warp < 8) {
-        registers_of_rows();
-        const int half = warp >> 2;
+    } else if (warp < ROW_WARPS) {
+        set_registers_up<104>();
+        const int part = warp >> 2;  // 32 columns (queries) of every tile
         const int key = (threadIdx.x & 127) + k0;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const float c = p.scale * LOG2E;
         bool ok = true;
         for (int it = 0; it < n; ++it) {
-            const int s = it % SHORT_STAGES, q0 = (i0 + it % per_head) * TILE + half * 64;
-            const float4* minus_lse = reinterpret_cast<const float4*>(stats + s * 2 * TILE + half * 64);
-            const float4* delta = minus_lse + TILE / 4;
-            float pr[64];
+            const int s = it % SHORT_STAGES, q0 = (i0 + it % per_head) * TILE + part * 32;
+            const float4* minus_lse = reinterpret_cast<const float4*>(stats + s * 2 * TILE + part * 32);
+            const float4* minus_delta = minus_lse + TILE / 4;
+            float pr[32], dp[32];
+            uint32_t pk[16];
             ok = __all_sync(0xffffffffu, mbar_wait(st_full + 8 * s, (it / SHORT_STAGES) & 1, wc) && mbar_wait(s_full, it & 1, wc));
             if (!ok)
                 break;
             tc_fence_after();
-            half_row(t_s + half * 64 + lanes, [&](int e, float x) { pr[e] = x; });
+            load_quarter(t_a + part * 32 + lanes, pr);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(s_free);
 #pragma unroll
-            for (int e = 0; e < 64; e += 4) {
+            for (int e = 0; e < 32; e += 4) {
                 const float4 z = minus_lse[e / 4];
                 Pair a = f32x2::fma({pr[e], pr[e + 1]}, both(c), {z.x, z.y});
                 Pair b = f32x2::fma({pr[e + 2], pr[e + 3]}, both(c), {z.z, z.w});
@@ -979,31 +1064,40 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             }
             if (p.causal && it % per_head == 0) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e)
+                for (int e = 0; e < 32; ++e)
                     if (q0 + e < key)
                         pr[e] = 0.f;
             }
-            uint32_t pk[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 16; ++e)
                 pk[e] = pack2<FP16>(pr[2 * e], pr[2 * e + 1]);
-            tmem_st_x32(t_s + half * 64 + lanes, pk);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0)
-                mbar_arrive(p_ready);
+            // (dV of the block before, which reads the last P, came before dP)
             ok = __all_sync(0xffffffffu, mbar_wait(dp_full, it & 1, wc));
             if (!ok)
                 break;
             tc_fence_after();
-            half_row(t_dp + half * 64 + lanes, [&](int e, float dp) {
-                const float4 d = delta[e / 4];
-                pr[e] *= dp - (e % 4 == 0 ? d.x : e % 4 == 1 ? d.y : e % 4 == 2 ? d.z : d.w);
-                if (e & 1)
-                    pk[e / 2] = pack2<FP16>(pr[e - 1], pr[e]);
-            });
-            tmem_st_x32(t_dp + half * 64 + lanes, pk);
+            tmem_st_x16(t_p + part * 16 + lanes, pk);
+            load_quarter(t_a + part * 32 + lanes, dp);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(dp_free);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+                const float4 d = minus_delta[e / 4];
+                const Pair a = f32x2::mul({pr[e], pr[e + 1]}, f32x2::add({dp[e], dp[e + 1]}, {d.x, d.y}));
+                const Pair b = f32x2::mul({pr[e + 2], pr[e + 3]}, f32x2::add({dp[e + 2], dp[e + 3]}, {d.z, d.w}));
+                pk[e / 2] = pack2<FP16>(a.x, a.y);
+                pk[e / 2 + 1] = pack2<FP16>(b.x, b.y);
+            }
+            if (it > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(dk_done, (it - 1) & 1, wc));
+                if (!ok)
+                    break;
+                tc_fence_after();
+            }
+            tmem_st_x16(t_ds + part * 16 + lanes, pk);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -1016,18 +1110,19 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             tc_fence_after();
             const bool live = key < w.len;
             const int64_t at = w.start + static_cast<int64_t>(key);
-            if (half == 0)
-                store_row<FP16>(t_dk + lanes, p.dim, p.scale, p.out0 + at * p.row0 + kv_head * p.head0, live);
+            const int from = (part & 1) * (DP / 2), to = (part & 1) ? p.dim : min(p.dim, DP / 2);
+            if (part < 2)
+                store_row<FP16>(t_dk + lanes, from, to, p.scale, p.out0 + at * p.row0 + kv_head * p.head0, live);
             else
-                store_row<FP16>(t_dv + lanes, p.dim, 1.f, p.out1 + at * p.row1 + kv_head * p.head1, live);
+                store_row<FP16>(t_dv + lanes, from, to, 1.f, p.out1 + at * p.row1 + kv_head * p.head1, live);
         }
     } else {
-        registers_of_others();
+        set_registers_down<64>();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8)
+    if (warp == MMA_WARP)
         tmem_dealloc_cg1(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
         *p.error_flag = 1;
