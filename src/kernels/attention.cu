@@ -191,13 +191,11 @@ __device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint32_t b
         if (kk < ksteps)
             umma_ss(d, a + step_k(kk), b + step_k(kk), idesc, kk != 0);
 }
-// [128, dim] (+)= P tile over the tile's 128 rows; WIDTH scores (32, 64 or 128) of a row were written by one thread,
-// where they were
-template <int WIDTH>
+// [128, dim] (+)= P tile over the tile's 128 rows
 __device__ __forceinline__ void multiply_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
 #pragma unroll
     for (int kk = 0; kk < TILE / 16; ++kk)
-        umma_ts(d, a + kk / (WIDTH / 16) * WIDTH + kk % (WIDTH / 16) * 8, b + step_mn(kk), idesc, kk != 0 || accumulate);
+        umma_ts(d, a + 8 * kk, b + step_mn(kk), idesc, kk != 0 || accumulate);
 }
 // A wait of the thread that issues products: it polls a while before it sleeps, which wakes it sooner
 __device__ __forceinline__ bool issue_wait(uint32_t bar, uint32_t parity, const WaitCtx& w) {
@@ -331,9 +329,11 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int from, int to, floa
 // ================================================================ forward
 //
 // A CTA takes two tiles of 128 queries of one head and walks over the keys once; while one warpgroup works on the
-// scores of its tile, the tensor cores work for the other tile.  The running maximum only moves when the
-// new one is more than 2^8 larger (then the accumulator is rescaled in TMEM by the threads that own its rows): P
-// stays below 2^8, which changes nothing in its relative precision, and the rescaling is rare.
+// scores of its tile, a row a thread, the tensor cores work for the other tile.  The running maximum is that of the
+// first block until a later one is more than 2^32 larger (2^8 for float16, whose numbers end at 2^16): P may
+// then be that large, which changes nothing in its relative precision.  So a block's exponentials do not wait for its
+// maximum, which is found beside them; only if it did rise that far they are taken again, and the threads that own its
+// rows rescale the accumulator in TMEM.
 constexpr int FWD_ROW_WARPS = 8, FWD_MMA = 8, FWD_TMA = 9;  // (and two warps that idle)
 constexpr int FWD_THREADS = 32 * (FWD_ROW_WARPS + 4);
 constexpr int FWD_STAGES = 4;
@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                     const bool last = j + 1 == n_blocks[t];
                     if (!last && !k_here)  // (asked for early: its answer comes while the products are issued)
                         k_here = mbar_test_wait(full0 + 8 * sk, pk);
-                    multiply_scores<TILE>(t_o + t * TILE, t_s + t * TILE, v, id_o, j != 0);
+                    multiply_scores(t_o + t * TILE, t_s + t * TILE, v, id_o, j != 0);
                     if (last) {
                         umma_commit_cg1(o_full + 8 * t);
                     } else {
@@ -512,68 +512,82 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         const int limit = p.causal ? min(w.len, row + 1) : w.len;  // keys that this row sees
         float m = 0.f, l = 0.f;
         bool ok = true;
+        // 32 scores of this row, masked
+        auto chunk = [&](uint32_t (&s)[32], int i, int k0, bool masked) {
+            tmem_ld_wait(s);
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (k0 + 32 * i + e >= limit)
+                        s[e] = 0xff800000u;
+            }
+        };
         for (int j = 0; j < n_blocks[t]; ++j) {
             ok = __all_sync(0xffffffffu, mbar_wait(s_full + 8 * t, j & 1, wc));
             if (!ok)
                 break;
             tc_fence_after();
-            uint32_t s[4][32];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                tmem_ld_32x32b_x32(s_at + 32 * i, s[i]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                tmem_ld_wait(s[i]);
             const int k0 = j * TILE;
-            if (k0 + TILE > w.len || (p.causal && k0 + TILE > r0 + t * TILE)) {
+            const bool masked = k0 + TILE > w.len || (p.causal && k0 + TILE > r0 + t * TILE);
+            uint32_t s[2][32], pk[2][32];
+            Pair sum[2];
+            // P with the maximum as it is, the block's own maximum beside it; a chunk is loaded while one is worked on
+            auto exponentials = [&]() {
+                const Pair cc = both(c), mc = both(-m * c);
+                float top[2] = {-INFINITY, -INFINITY};
+                sum[0] = sum[1] = both(0.f);
+                tmem_ld_32x32b_x32(s_at, s[0]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
+                    chunk(s[i & 1], i, k0, masked);
+                    if (i < 3)
+                        tmem_ld_32x32b_x32(s_at + 32 * (i + 1), s[(i + 1) & 1]);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (k0 + 32 * i + e >= limit)
-                            s[i][e] = 0xff800000u;
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < 32; e += 2)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    top[i] = max3_nan(top[i], __uint_as_float(s[i][e]), __uint_as_float(s[i][e + 1]));
-            const float mx = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
-            // each row goes by its own maximum (also where a score is NaN: the row becomes NaN)
-            const bool rises = !((mx - m) * c <= 8.f) && row < w.len;
+                    for (int e = 0; e < 16; ++e) {
+                        const float a = __uint_as_float(s[i & 1][2 * e]), b = __uint_as_float(s[i & 1][2 * e + 1]);
+                        Pair x = f32x2::fma({a, b}, cc, mc);
+                        x = e % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
+                        top[e & 1] = max3_nan(top[e & 1], a, b);
+                        sum[e & 1] = f32x2::add(sum[e & 1], x);
+                        pk[i / 2][16 * (i & 1) + e] = pack2<FP16>(x.x, x.y);
+                    }
+                }
+                return max3_nan(top[0], top[1], top[1]);
+            };
             if (j == 0) {
-                m = mx;
-            } else if (__any_sync(0xffffffffu, rises)) {
-                // the product that last added to O has retired: the scores' barrier came after it
-                const float to = rises ? max3_nan(m, mx, mx) : m, f = ex2((m - to) * c);
-                m = to;
-                l *= f;
-                for (int d = 0; d < p.dim; d += 32) {
-                    uint32_t o[32];
-                    tmem_ld_32x32b_x32(o_at + d, o);
-                    tmem_ld_wait(o);
+                float top = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    tmem_st_x32(o_at + d, o);
+                for (int i = 0; i < 4; ++i) {
+                    tmem_ld_32x32b_x32(s_at + 32 * i, s[0]);
+                    chunk(s[0], i, k0, masked);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2)
+                        top = max3_nan(top, __uint_as_float(s[0][e]), __uint_as_float(s[0][e + 1]));
+                }
+                m = top;
+                exponentials();
+            } else {
+                const float mx = exponentials();
+                // each row goes by its own maximum (also where a score is NaN: the row becomes NaN)
+                const bool rises = !((mx - m) * c <= (FP16 ? 8.f : 32.f)) && row < w.len;
+                if (__any_sync(0xffffffffu, rises)) {
+                    // the product that last added to O has retired: the scores' barrier came after it
+                    const float to = rises ? max3_nan(m, mx, mx) : m, f = ex2((m - to) * c);
+                    m = to;
+                    l *= f;
+                    for (int d = 0; d < p.dim; d += 32) {
+                        tmem_ld_32x32b_x32(o_at + d, s[0]);
+                        tmem_ld_wait(s[0]);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * f);
+                        tmem_st_x32(o_at + d, s[0]);
+                    }
+                    exponentials();
                 }
             }
-            const Pair cc = both(c), mc = both(-m * c);
-            Pair sum[2] = {both(0.f), both(0.f)};
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t pk[32];
-#pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    const uint32_t* at = &s[2 * h + e / 16][2 * (e % 16)];
-                    Pair x = f32x2::fma({__uint_as_float(at[0]), __uint_as_float(at[1])}, cc, mc);
-                    x = e % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
-                    sum[e & 1] = f32x2::add(sum[e & 1], x);
-                    pk[e] = pack2<FP16>(x.x, x.y);
-                }
-                tmem_st_x32(s_at + 32 * h, pk);
-            }
+            tmem_st_x32(s_at, pk[0]);
+            tmem_st_x32(s_at + 32, pk[1]);
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             tmem_st_wait();
             tc_fence_before();
@@ -630,8 +644,9 @@ __global__ void __launch_bounds__(256) delta_kernel(const uint16_t* __restrict__
 // ================================================================ backward: dQ
 //
 // A CTA takes 128 queries of one head.  All row warps work on every tile of scores, a thread on a quarter of a row.
-//   tensor cores:  S(j+1)         dQ += dS(j) K, dP(j+1) = dO V^T      S(j+2) ...
-//   row warps:     dS(j) from dP  P(j+1) from S                        dS(j+1) ...
+// Each has its own region of TMEM, which is free again as soon as its reader holds it in registers:
+//   tensor cores:  S(j+1), dP(j+1) = dO V^T, dQ += dS(j) K, ...
+//   row warps:     P(j) from S(j), dS(j) from dP(j), ...
 constexpr int ROW_WARPS = 16, MMA_WARP = 16, TMA_WARP = 17, STAT_WARP = 18;  // (and a warp that idles)
 constexpr int BWD_THREADS = 32 * (ROW_WARPS + 4);  // 512 x 104 + 128 x 64 = 640 x 96 registers
 
@@ -665,9 +680,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring_v + SHORT_STAGES * TB);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8 * LONG_STAGES, v_full = k_empty + 8 * LONG_STAGES,
                    v_empty = v_full + 8 * SHORT_STAGES;
-    const uint32_t q_full = v_empty + 8 * SHORT_STAGES, s_full = q_full + 8, s_free = s_full + 8, dp_full = s_free + 8, ds_ready = dp_full + 8,
-                   done = ds_ready + 8, side = done + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (LONG_STAGES + SHORT_STAGES) + 7);
+    const uint32_t q_full = v_empty + 8 * SHORT_STAGES, s_full = q_full + 8, s_free = s_full + 8, dp_full = s_free + 8, dp_free = dp_full + 8,
+                   ds_ready = dp_free + 8, dq_done = ds_ready + 8, done = dq_done + 8, side = done + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * (LONG_STAGES + SHORT_STAGES) + 9);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     Where* where = reinterpret_cast<Where*>(tmem_slot + 2);
 
@@ -687,6 +702,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         mbar_init(s_full, 1);
         mbar_init(s_free, ROW_WARPS);
         mbar_init(dp_full, 1);
+        mbar_init(dp_free, ROW_WARPS);
+        mbar_init(dq_done, 1);
         mbar_init(ds_ready, ROW_WARPS);
         mbar_init(done, 1);
         mbar_init(side, 1);
@@ -705,7 +722,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dq = tmem + 2 * TILE;
+    const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dq = tmem + 2 * TILE, t_ds = tmem + 3 * TILE;
     const int r0 = (w.tiles - 1 - w.local) * TILE;
     const int keys = p.causal ? min(w.len, r0 + TILE) : w.len;
     const int n = (keys + TILE - 1) / TILE;
@@ -754,21 +771,25 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 umma_commit_cg1(v_empty + 8 * s);
                 return true;
             };
+            auto k_here = [&](int j) { return mbar_test_wait(k_full + 8 * (j % LONG_STAGES), (j / LONG_STAGES) & 1); };
+            auto v_here = [&](int j) { return mbar_test_wait(v_full + 8 * (j % SHORT_STAGES), (j / SHORT_STAGES) & 1); };
             bool ok = issue_wait(q_full, 0, wc) && scores(0, false) && grads(0, false);
             for (int j = 0; ok && j < n; ++j) {
-                if (j + 1 < n) {
-                    const bool here = mbar_test_wait(k_full + 8 * ((j + 1) % LONG_STAGES), ((j + 1) / LONG_STAGES) & 1);
-                    ok = issue_wait(s_free, j & 1, wc) && scores(j + 1, here);
-                }
-                ok = ok && issue_wait(ds_ready, j & 1, wc);
+                const bool more = j + 1 < n, k_now = more && k_here(j + 1);
+                if (more)
+                    ok = issue_wait(s_free, j & 1, wc) && scores(j + 1, k_now);
+                const bool v_now = more && v_here(j + 1);
+                ok = ok && issue_wait(dp_free, j & 1, wc);
+                const bool ds_now = ok && mbar_test_wait(ds_ready, j & 1);
+                if (ok && more)
+                    ok = grads(j + 1, v_now);
+                ok = ok && (ds_now || issue_wait(ds_ready, j & 1, wc));
                 if (!ok)
                     break;
                 tc_fence_after();
-                const bool here = j + 1 < n && mbar_test_wait(v_full + 8 * ((j + 1) % SHORT_STAGES), ((j + 1) / SHORT_STAGES) & 1);
-                multiply_scores<32>(t_dq, t_dp, desc_mn(k0 + j % LONG_STAGES * TB), id_d, j != 0);
+                multiply_scores(t_dq, t_ds, desc_mn(k0 + j % LONG_STAGES * TB), id_d, j != 0);
                 umma_commit_cg1(k_empty + 8 * (j % LONG_STAGES));
-                if (j + 1 < n)
-                    ok = grads(j + 1, here);
+                umma_commit_cg1(dq_done);
             }
             if (ok)
                 umma_commit_cg1(done);
@@ -815,13 +836,23 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 break;
             tc_fence_after();
             load_quarter(t_dp + part * 32 + lanes, dp);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0)
+                mbar_arrive(dp_free);
             uint32_t pk[16];
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
                 const Pair x = f32x2::mul({pr[e], pr[e + 1]}, f32x2::add({dp[e], dp[e + 1]}, both(-delta)));
                 pk[e / 2] = pack2<FP16>(x.x, x.y);
             }
-            tmem_st_x16(t_dp + part * 32 + lanes, pk);
+            if (j > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait(dq_done, (j - 1) & 1, wc));
+                if (!ok)
+                    break;
+                tc_fence_after();
+            }
+            tmem_st_x16(t_ds + part * 16 + lanes, pk);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -951,10 +982,18 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 break;
             float* to = stats + s * 2 * TILE;
             const int64_t at = static_cast<int64_t>(head) * p.tokens + w.start + q0;
-            for (int r = lane; r < TILE; r += 32) {
+            float z[TILE / 32], d[TILE / 32];
+#pragma unroll
+            for (int i = 0; i < TILE / 32; ++i) {
+                const int r = lane + 32 * i;
                 const bool live = q0 + r < w.len;
-                to[r] = live ? p.lse[at + r] * -LOG2E : -INFINITY;
-                to[TILE + r] = live ? -p.delta[at + r] : 0.f;
+                z[i] = live ? p.lse[at + r] : INFINITY;
+                d[i] = live ? p.delta[at + r] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < TILE / 32; ++i) {
+                to[lane + 32 * i] = z[i] * -LOG2E;
+                to[TILE + lane + 32 * i] = -d[i];
             }
             __syncwarp();
             if (lane == 0)
@@ -989,7 +1028,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             // (P is in place when dP has been read: both are told by one barrier)
             auto add_dv = [&](int it) {
                 const int s = it % SHORT_STAGES;
-                multiply_scores<TILE>(t_dv, t_p, desc_mn(ro + s * TB), id_d, it != 0);
+                multiply_scores(t_dv, t_p, desc_mn(ro + s * TB), id_d, it != 0);
                 umma_commit_cg1(o_empty + 8 * s);
             };
             auto add_dk = [&](int it, bool here) {
@@ -997,7 +1036,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 if (!here && !issue_wait(ds_ready, it & 1, wc))
                     return false;
                 tc_fence_after();
-                multiply_scores<TILE>(t_dk, t_ds, desc_mn(rq + s * TB), id_d, it != 0);
+                multiply_scores(t_dk, t_ds, desc_mn(rq + s * TB), id_d, it != 0);
                 umma_commit_cg1(q_empty + 8 * s);
                 umma_commit_cg1(dk_done);
                 return true;
