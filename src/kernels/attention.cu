@@ -118,6 +118,10 @@ template <int N>
 __device__ __forceinline__ void set_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void set_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// Programmatic launches: the next kernel of the stream may start once all CTAs of this one have said so (or ended);
+// it waits where it needs this one's end.
+__device__ __forceinline__ void next_kernel_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_last_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -621,6 +625,7 @@ template <bool FP16>
 __global__ void __launch_bounds__(256) delta_kernel(const uint16_t* __restrict__ out, int64_t o_row, int64_t o_head,
                                                     const uint16_t* __restrict__ dout, int64_t d_row, int64_t d_head, int tokens,
                                                     int heads, int dim, float* __restrict__ delta) {
+    next_kernel_may_start();
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4);  // half a warp a row
     const int sub = threadIdx.x & 15;
     const int64_t row = i / heads, head = i % heads;
@@ -674,8 +679,10 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     constexpr int TB = tile_bytes<DP>();
     extern __shared__ __align__(1024) uint8_t smem[];  // Q, dO, then K slots, then V slots
-    if (unaligned(smem, p))
+    if (unaligned(smem, p)) {
+        wait_for_last_kernel();
         return;
+    }
     uint8_t *ring_k = smem + 2 * TB, *ring_v = ring_k + LONG_STAGES * TB;
     uint64_t* bars = reinterpret_cast<uint64_t*>(ring_v + SHORT_STAGES * TB);
     const uint32_t k_full = smem_u32(bars), k_empty = k_full + 8 * LONG_STAGES, v_full = k_empty + 8 * LONG_STAGES,
@@ -712,8 +719,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     }
     __syncthreads();
     const Where w = *where;
-    if (w.len == 0)
+    // The kernel before, dK and dV, need not have ended for this one to work, which fills the processors that it leaves
+    // idle towards its end; but what comes after this one relies on both: its last CTA waits.
+    const bool ends_last = blockIdx.x == gridDim.x - 1;
+    if (w.len == 0) {
+        if (ends_last)
+            wait_for_last_kernel();
         return;
+    }
     if (warp == MMA_WARP) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
@@ -874,6 +887,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         tmem_dealloc_cg1(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
         *p.error_flag = 1;
+    if (ends_last)
+        wait_for_last_kernel();
 }
 
 // ================================================================ backward: dK and dV
@@ -975,6 +990,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         }
     } else if (warp == STAT_WARP) {
         set_registers_down<64>();
+        // delta has to be complete; and only then may dQ start, which relies on that
+        wait_for_last_kernel();
+        next_kernel_may_start();
         // -lse log2 e and -delta of every block's rows; a row behind the end has probabilities of zero
         for (int it = 0; it < n; ++it) {
             const int s = it % SHORT_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
@@ -1224,14 +1242,25 @@ cudaError_t pick(const Problem& p, F go) {
     return p.fp16 ? go(std::integral_constant<int, 128>{}, T{}) : go(std::integral_constant<int, 128>{}, N{});
 }
 // (the attribute belongs to a function on a device: it is set before every launch, which costs under a microsecond)
-template <class K, class... A>
-cudaError_t run(K kernel, unsigned grid, int threads, int smem, cudaStream_t stream, A... args) {
+// `early`: the kernel may start before the one in front of it has ended
+template <class... P, class... A>
+cudaError_t run(void (*kernel)(P...), unsigned grid, int threads, int smem, bool early, cudaStream_t stream, const A&... args) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess)
         return e;
-    kernel<<<grid, threads, smem, stream>>>(args...);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = threads;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = early ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, args...);
     count_launch();
-    return cudaGetLastError();
+    return e;
 }
 
 }  // namespace
@@ -1254,7 +1283,7 @@ cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tenso
     a.lse = lse;
     return pick(p, [&](auto dp, auto half) {
         constexpr int DP = decltype(dp)::value;
-        return run(forward_kernel<DP, decltype(half)::value>, grid, FWD_THREADS, fwd_smem<DP>(), stream, mq, mk, mv, a);
+        return run(forward_kernel<DP, decltype(half)::value>, grid, FWD_THREADS, fwd_smem<DP>(), false, stream, mq, mk, mv, a);
     });
 }
 
@@ -1295,13 +1324,13 @@ cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, T
         a.out1 = static_cast<uint16_t*>(dv.p);
         a.row1 = dv.row;
         a.head1 = dv.head;
-        const cudaError_t first = run(dkv_kernel<DP, FP16>, grid_k, BWD_THREADS, bwd_smem<DP>(), stream, mq, mk, mv, mo, a);
+        const cudaError_t first = run(dkv_kernel<DP, FP16>, grid_k, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
         if (first != cudaSuccess)
             return first;
         a.out0 = static_cast<uint16_t*>(dq.p);
         a.row0 = dq.row;
         a.head0 = dq.head;
-        return run(dq_kernel<DP, FP16>, grid_q, BWD_THREADS, bwd_smem<DP>(), stream, mq, mk, mv, mo, a);
+        return run(dq_kernel<DP, FP16>, grid_q, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
     });
 }
 
