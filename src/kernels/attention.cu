@@ -352,6 +352,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
         forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const Params p) {
     constexpr int TB = tile_bytes<DP>();
+    // the last tiles of a sequence, which have the most keys, come first
+    auto first_row = [](const Where& w) { return (w.tiles - 1 - w.local) * 2 * TILE; };
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* ring = smem + 2 * TB;
@@ -366,44 +368,52 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const int head = static_cast<int>(blockIdx.x % p.heads);
-    if (warp == 0) {
-        const Where w = find_tile(p, 2 * TILE, static_cast<int>(blockIdx.x / p.heads));
-        if (lane == 0)
-            *where = w;
-    }
-    if (warp == FWD_TMA && lane == 0) {
-        *abort_flag = 0;
-        for (int s = 0; s < 2 * FWD_STAGES; ++s)
-            mbar_init(full0 + 8 * s, 1);
-        for (int t = 0; t < 2; ++t) {
-            mbar_init(q_full + 8 * t, 1);
-            mbar_init(s_full + 8 * t, 1);
-            mbar_init(p_ready + 8 * t, FWD_ROW_WARPS / 2);
-            mbar_init(o_full + 8 * t, 1);
+    const int kv_head = head / (p.heads / p.kv_heads);
+    if (warp == FWD_TMA) {
+        if (lane == 0) {
+            *abort_flag = 0;
+            for (int s = 0; s < 2 * FWD_STAGES; ++s)
+                mbar_init(full0 + 8 * s, 1);
+            for (int t = 0; t < 2; ++t) {
+                mbar_init(q_full + 8 * t, 1);
+                mbar_init(s_full + 8 * t, 1);
+                mbar_init(p_ready + 8 * t, FWD_ROW_WARPS / 2);
+                mbar_init(o_full + 8 * t, 1);
+            }
+            mbar_init(side, 1);
+            mbar_fence_init();
+            fence_proxy_async_smem();
         }
-        mbar_init(side, 1);
-        mbar_fence_init();
-        fence_proxy_async_smem();
-        prefetch_tensormap(&map_q);
-        prefetch_tensormap(&map_k);
-        prefetch_tensormap(&map_v);
-    }
-    __syncthreads();
-    const Where w = *where;
-    if (w.len == 0)
-        return;  // all threads alike, before anything is allocated
-    if (warp == FWD_MMA) {
+        const Where found = find_tile(p, 2 * TILE, static_cast<int>(blockIdx.x / p.heads));
+        __syncwarp();
+        if (elect_one()) {
+            *where = found;
+            if (found.len > 0) {  // the first copies are under way while the rest is set up
+                const int first = first_row(found);
+                load_tile<DP>(smem_u32(smem), &map_q, q_full, head, found.start + first);
+                load_tile<DP>(smem_u32(ring), &map_k, full0, kv_head, found.start);
+                if (first + TILE < found.len)
+                    load_tile<DP>(smem_u32(smem) + TB, &map_q, q_full + 8, head, found.start + first + TILE);
+            }
+        }
+        __syncwarp();
+    } else if (warp == FWD_MMA) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const Where w = *where;
     const uint32_t tmem = *tmem_slot;
+    if (w.len == 0) {  // no such tile
+        if (warp == FWD_MMA)
+            tmem_dealloc_cg1(tmem, 512);
+        return;
+    }
     const uint32_t t_s = tmem, t_o = tmem + 2 * TILE;  // S of tile t at t_s + 128 t, O at t_o + 128 t
 
-    // the last tiles of a sequence, which have the most keys, come first
-    const int r0 = (w.tiles - 1 - w.local) * 2 * TILE;
+    const int r0 = first_row(w);
     int n_blocks[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -416,15 +426,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 
     if (warp == FWD_TMA) {
         set_registers_down<72>();  // 256 x 216 + 128 x 72 = 384 x 168
-        const int kv_head = head / (p.heads / p.kv_heads);
-        if (elect_one()) {
-            load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
-            if (n_blocks[1] > 0)
-                load_tile<DP>(smem_u32(smem) + TB, &map_q, q_full + 8, head, w.start + r0 + TILE);
-        }
-        __syncwarp();
         uint32_t side_phase = 0;
-        for (int it = 0; it < 2 * n; ++it) {
+        for (int it = 1; it < 2 * n; ++it) {  // (0 is on its way)
             const int s = it % FWD_STAGES;
             if (!__all_sync(0xffffffffu, mbar_wait(empty0 + 8 * s, ((it / FWD_STAGES) & 1) ^ 1, wc)))
                 break;
@@ -678,6 +681,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                   const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do, const Params p) {
     constexpr int TB = tile_bytes<DP>();
+    // the last tiles of a sequence, which have the most keys, come first
+    auto first_row = [](const Where& w) { return (w.tiles - 1 - w.local) * TILE; };
     extern __shared__ __align__(1024) uint8_t smem[];  // Q, dO, then K slots, then V slots
     if (unaligned(smem, p)) {
         wait_for_last_kernel();
@@ -696,59 +701,61 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
     const int head = static_cast<int>(blockIdx.x % p.heads);
-    if (warp == 0) {
-        const Where w = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.heads));
-        if (lane == 0)
-            *where = w;
-    }
-    if (warp == TMA_WARP && lane == 0) {
-        *abort_flag = 0;
-        for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
-            mbar_init(k_full + 8 * s, 1);
-        mbar_init(q_full, 2);
-        mbar_init(s_full, 1);
-        mbar_init(s_free, ROW_WARPS);
-        mbar_init(dp_full, 1);
-        mbar_init(dp_free, ROW_WARPS);
-        mbar_init(dq_done, 1);
-        mbar_init(ds_ready, ROW_WARPS);
-        mbar_init(done, 1);
-        mbar_init(side, 1);
-        mbar_fence_init();
-        fence_proxy_async_smem();
-    }
-    __syncthreads();
-    const Where w = *where;
-    // The kernel before, dK and dV, need not have ended for this one to work, which fills the processors that it leaves
-    // idle towards its end; but what comes after this one relies on both: its last CTA waits.
-    const bool ends_last = blockIdx.x == gridDim.x - 1;
-    if (w.len == 0) {
-        if (ends_last)
-            wait_for_last_kernel();
-        return;
-    }
-    if (warp == MMA_WARP) {
+    const int kv_head = head / (p.heads / p.kv_heads);
+    if (warp == TMA_WARP) {
+        if (lane == 0) {
+            *abort_flag = 0;
+            for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
+                mbar_init(k_full + 8 * s, 1);
+            mbar_init(q_full, 2);
+            mbar_init(s_full, 1);
+            mbar_init(s_free, ROW_WARPS);
+            mbar_init(dp_full, 1);
+            mbar_init(dp_free, ROW_WARPS);
+            mbar_init(dq_done, 1);
+            mbar_init(ds_ready, ROW_WARPS);
+            mbar_init(done, 1);
+            mbar_init(side, 1);
+            mbar_fence_init();
+            fence_proxy_async_smem();
+        }
+        const Where found = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.heads));
+        __syncwarp();
+        if (elect_one()) {
+            *where = found;
+            if (found.len > 0) {  // the first copies are under way while the rest is set up
+                load_tile<DP>(smem_u32(smem), &map_q, q_full, head, found.start + first_row(found));
+                load_tile<DP>(smem_u32(smem) + TB, &map_do, q_full, head, found.start + first_row(found));
+            }
+        }
+        __syncwarp();
+    } else if (warp == MMA_WARP) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const Where w = *where;
+    // The kernel before, dK and dV, need not have ended for this one to work, which fills the processors that it leaves
+    // idle towards its end; but what comes after this one relies on both: its last CTA waits.
+    const bool ends_last = blockIdx.x == gridDim.x - 1;
     const uint32_t tmem = *tmem_slot;
+    if (w.len == 0) {  // no such tile
+        if (warp == MMA_WARP)
+            tmem_dealloc_cg1(tmem, 512);
+        if (ends_last)
+            wait_for_last_kernel();
+        return;
+    }
     const uint32_t t_s = tmem, t_dp = tmem + TILE, t_dq = tmem + 2 * TILE, t_ds = tmem + 3 * TILE;
-    const int r0 = (w.tiles - 1 - w.local) * TILE;
+    const int r0 = first_row(w);
     const int keys = p.causal ? min(w.len, r0 + TILE) : w.len;
     const int n = (keys + TILE - 1) / TILE;
     WaitCtx wc{abort_flag, WAIT_NS};
 
     if (warp == TMA_WARP) {
         set_registers_down<64>();
-        const int kv_head = head / (p.heads / p.kv_heads);
-        if (elect_one()) {
-            load_tile<DP>(smem_u32(smem), &map_q, q_full, head, w.start + r0);
-            load_tile<DP>(smem_u32(smem) + TB, &map_do, q_full, head, w.start + r0);
-        }
-        __syncwarp();
         uint32_t side_phase = 0;
         for (int j = 0; j < n; ++j) {
             const int s = j % LONG_STAGES, sv = j % SHORT_STAGES, live = w.len - j * TILE;
@@ -926,43 +933,51 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const int lane = threadIdx.x & 31;
     const int kv_head = static_cast<int>(blockIdx.x % p.kv_heads);
     const int group = p.heads / p.kv_heads;
-    if (warp == 0) {
-        const Where w = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.kv_heads));
-        if (lane == 0)
-            *where = w;
-    }
-    if (warp == TMA_WARP && lane == 0) {
-        *abort_flag = 0;
-        for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
-            mbar_init(q_full + 8 * s, 1);
-        for (int s = 0; s < SHORT_STAGES; ++s) {
-            mbar_init(st_full + 8 * s, 1);
-            mbar_init(st_empty + 8 * s, ROW_WARPS);
+    if (warp == TMA_WARP) {
+        if (lane == 0) {
+            *abort_flag = 0;
+            for (int s = 0; s < 2 * (LONG_STAGES + SHORT_STAGES); ++s)
+                mbar_init(q_full + 8 * s, 1);
+            for (int s = 0; s < SHORT_STAGES; ++s) {
+                mbar_init(st_full + 8 * s, 1);
+                mbar_init(st_empty + 8 * s, ROW_WARPS);
+            }
+            mbar_init(kv_full, 2);
+            mbar_init(s_full, 1);
+            mbar_init(s_free, ROW_WARPS);
+            mbar_init(dp_full, 1);
+            mbar_init(dp_free, ROW_WARPS);
+            mbar_init(ds_ready, ROW_WARPS);
+            mbar_init(dk_done, 1);
+            mbar_init(done, 1);
+            mbar_init(side, 1);
+            mbar_fence_init();
+            fence_proxy_async_smem();
         }
-        mbar_init(kv_full, 2);
-        mbar_init(s_full, 1);
-        mbar_init(s_free, ROW_WARPS);
-        mbar_init(dp_full, 1);
-        mbar_init(dp_free, ROW_WARPS);
-        mbar_init(ds_ready, ROW_WARPS);
-        mbar_init(dk_done, 1);
-        mbar_init(done, 1);
-        mbar_init(side, 1);
-        mbar_fence_init();
-        fence_proxy_async_smem();
-    }
-    __syncthreads();
-    const Where w = *where;
-    if (w.len == 0)
-        return;
-    if (warp == MMA_WARP) {
+        const Where found = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.kv_heads));
+        __syncwarp();
+        if (elect_one()) {
+            *where = found;
+            if (found.len > 0) {  // the first copies are under way while the rest is set up
+                load_tile<DP>(smem_u32(smem), &map_k, kv_full, kv_head, found.start + found.local * TILE);
+                load_tile<DP>(smem_u32(smem) + TB, &map_v, kv_full, kv_head, found.start + found.local * TILE);
+            }
+        }
+        __syncwarp();
+    } else if (warp == MMA_WARP) {
         tmem_alloc_cg1(smem_u32(tmem_slot), 512);
         tmem_relinquish_cg1();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const Where w = *where;
     const uint32_t tmem = *tmem_slot;
+    if (w.len == 0) {  // no such tile
+        if (warp == MMA_WARP)
+            tmem_dealloc_cg1(tmem, 512);
+        return;
+    }
     const uint32_t t_a = tmem, t_p = tmem + TILE, t_ds = t_p + 64, t_dv = tmem + 2 * TILE, t_dk = tmem + 3 * TILE;
     const int k0 = w.local * TILE;               // the first keys, which the most queries see, come first
     const int i0 = p.causal ? w.local : 0;       // first block of queries that sees them
@@ -972,11 +987,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 
     if (warp == TMA_WARP) {
         set_registers_down<64>();
-        if (elect_one()) {
-            load_tile<DP>(smem_u32(smem), &map_k, kv_full, kv_head, w.start + k0);
-            load_tile<DP>(smem_u32(smem) + TB, &map_v, kv_full, kv_head, w.start + k0);
-        }
-        __syncwarp();
         uint32_t side_phase = 0;
         for (int it = 0; it < n; ++it) {
             const int s = it % LONG_STAGES, so = it % SHORT_STAGES, head = kv_head * group + it / per_head;
