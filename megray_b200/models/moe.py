@@ -20,7 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import _lib
-from ..ops import EPI_DSWIGLU, EPI_SWIGLU, gemm, mse_loss_grad, sgd_step
+from ..ops import EPI_DSWIGLU, EPI_SWIGLU, AdamWState, adamw_step, balance_loss_grad, gemm, mse_loss_grad, sgd_step
 from ..ops.gemm import gemm_error_flag
 from ..parallel.expert_parallel import ExpertParallelOps
 from ..ops._stream import raw_stream
@@ -40,6 +40,9 @@ class MoEConfig:
     lr: float = 1e-4
     capacity_factor: float = 1.25
     seed: int = 0
+    balance_coef: float = 0.0    # weight of the router's balance loss, added to the loss
+    optimizer: str = "sgd"       # or "adamw", "adamw8" (moments in 8 bits)
+    weight_decay: float = 0.0    # of the AdamW steps
 
 
 class MoELayer:
@@ -51,6 +54,8 @@ class MoELayer:
         H, F, T = cfg.hidden, cfg.ffn, cfg.tokens
         if H % 256 or F % 128:
             raise ValueError("hidden must be a multiple of 256 and ffn of 128")
+        if cfg.optimizer not in ("sgd", "adamw", "adamw8"):
+            raise ValueError("optimizer is sgd, adamw or adamw8")
         self.ep = ExpertParallelOps(comm, T, H, cfg.experts, cfg.capacity_factor)
         El, cap = self.ep.El, self.ep.capacity
         bf = dict(dtype=torch.bfloat16, device=self.device)
@@ -78,6 +83,11 @@ class MoELayer:
         self.dx = torch.empty(T, H, **bf)
         self.dw = torch.empty(T, 2, dtype=torch.float32, device=self.device)
         self.dlogits = torch.empty(T, cfg.experts, dtype=torch.float32, device=self.device)
+        self.adamw = None if cfg.optimizer == "sgd" else AdamWState([self.w_gu, self.w_down],
+                                                                    bits=8 if cfg.optimizer == "adamw8" else 32)
+        self.steps = 0                                   # AdamW steps made
+        self.balance_loss = self.expert_counts = None    # of the last backward pass with a balance_coef
+        self._logits = None
         self.x_dev = torch.empty(T, H, **bf)
         self.logits_dev = torch.empty(T, cfg.experts, dtype=torch.float32, device=self.device)
 
@@ -121,6 +131,7 @@ class MoELayer:
 
     # ------------------------------------------------------------------ forward / backward
     def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        self._logits = logits if self.cfg.balance_coef else None  # read again by the backward pass
         ep, F, H = self.ep, self.cfg.ffn, self.cfg.hidden
         px, pl = plain(x, (ep.T, H)), plain(logits, (ep.T, ep.E), torch.float32)
         args = self._native_forward_args() if px and pl else None
@@ -142,7 +153,16 @@ class MoELayer:
         return self.out
 
     def backward(self, dout: torch.Tensor):
-        """Returns (dx, dlogits); fills the expert weight gradients."""
+        """Returns (dx, dlogits); fills the expert weight gradients.  With a ``balance_coef`` the gradient of the balance
+        loss over all ranks' tokens is added to ``dlogits``; ``balance_loss`` (one float32) and ``expert_counts`` hold
+        that loss and the pairs per expert."""
+        dx, dlogits = self._backward(dout)
+        if self.cfg.balance_coef:
+            self.balance_loss, self.expert_counts, _ = balance_loss_grad(
+                self._logits, self.ep.idx, self.cfg.balance_coef, dlogits=dlogits, accumulate=True, comm=self.comm)
+        return dx, dlogits
+
+    def _backward(self, dout: torch.Tensor):
         ep, F, H = self.ep, self.cfg.ffn, self.cfg.hidden
         pd = plain(dout, (ep.T, H))
         args = self._native_backward_args() if pd else None
@@ -168,6 +188,11 @@ class MoELayer:
         return self.dx, self.dlogits
 
     def optimizer_step(self) -> None:
+        if self.adamw is not None:
+            self.steps += 1
+            adamw_step([self.w_gu, self.w_down], [self.g_gu, self.g_down], self.adamw, self.cfg.lr, step=self.steps,
+                       weight_decay=self.cfg.weight_decay)
+            return
         sgd_step(self.w_gu, self.g_gu, self.cfg.lr)
         sgd_step(self.w_down, self.g_down, self.cfg.lr)
 
@@ -176,7 +201,7 @@ class MoELayer:
         loss, dy = mse_loss_grad(y, None, 1.0 / (self.cfg.tokens * self.n * self.cfg.hidden))
         self.backward(dy)
         self.optimizer_step()
-        return loss
+        return loss + self.balance_loss if self.cfg.balance_coef else loss
 
     def train_step(self, x_host: torch.Tensor, logits_host: torch.Tensor) -> float:
         """Public call: tokens and router logits come from pinned host memory, the loss goes back."""

@@ -18,7 +18,7 @@ from ._stream import raw_stream
 
 BLOCK = 256
 _CODES = {torch.float32: 7, torch.bfloat16: 10}
-_RECORD = np.dtype([("p", "u8"), ("g", "u8"), ("copy", "u8"), ("n", "u8"), ("block", "u8")])
+_P, _G, _COPY, _N, _BLOCK_AT = range(5)  # columns of megray_adamw_tensor
 
 
 # (called once per tensor: as C functions on a list, which is what a long one costs on the host)
@@ -44,8 +44,8 @@ class AdamWState:
         blocks = np.array([-(-n // BLOCK) for n in self.sizes], dtype=np.uint64)
         first = np.cumsum(blocks) - blocks
         self.begins = [int(b) * BLOCK for b in first]
-        self._records = np.zeros(len(params), dtype=_RECORD)
-        self._records["n"], self._records["block"] = self.sizes, first
+        self._records = np.zeros((len(params), 5), dtype=np.uint64)
+        self._records[:, _N], self._records[:, _BLOCK_AT] = self.sizes, first
         total = int(blocks.sum())
         if bits == 32:
             self.m, self.v = (torch.zeros(total * BLOCK, dtype=torch.float32, device=self.device) for _ in range(2))
@@ -86,8 +86,7 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
     float32 tensors of one element on the device: a captured graph then follows their contents, while host numbers
     are part of the capture."""
     n = len(state.sizes)
-    params, grads = list(params), list(grads)
-    copies = list(copies) if copies is not None else None
+    params, grads, copies = list(params), list(grads), None if copies is None else list(copies)
     if len(params) != n or len(grads) != n or (copies is not None and len(copies) != n):
         raise ValueError("adamw_step: expected as many parameters, gradients and copies as the state was made with")
     device = state.device
@@ -117,26 +116,27 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
         params, grads = [params[i] for i in keep], [grads[i] for i in keep]
         copies = [copies[i] for i in keep] if copies is not None else None
         records, sizes = records[keep], [sizes[i] for i in keep]
-    records = records.copy()
-    for name, field, ts, types in (("parameter", "p", params, _CODES), ("gradient", "g", grads, _CODES),
-                                   ("copy", "copy", copies or [], (torch.bfloat16,))):
+    records, one_kind = records.copy(), True
+    for name, field, ts, types in (("parameter", _P, params, _CODES), ("gradient", _G, grads, _CODES),
+                                   ("copy", _COPY, copies or [], (torch.bfloat16,))):
         if not ts:
             continue
         kinds = set(map(_dtype, ts))
+        one_kind = one_kind and len(kinds) == 1
         if not kinds.issubset(types):
             raise ValueError(f"adamw_step: a {name} is {kinds}; float32 and bf16 are taken, bf16 alone for copies")
         if (list(map(_numel, ts)) != sizes or set(map(_device, ts)) != {device.index} or
                 not all(map(_contiguous, ts))):
             raise ValueError(f"adamw_step: a {name} has another size than its parameter had when the state was made, "
                              "is not contiguous or lies on another device")
-        records[field] = np.fromiter(map(_address, ts), dtype=np.uint64, count=len(ts))
-    lib, stream = _lib.load(), raw_stream()
-    kinds = set(zip(map(_dtype, params), map(_dtype, grads)))
-    for kind in kinds:
-        part = records
-        if len(kinds) > 1:
-            part = records[[(p.dtype, g.dtype) == kind for p, g in zip(params, grads)]]
-        args.p_dtype, args.g_dtype = _CODES[kind[0]], _CODES[kind[1]]
-        rc = lib.megray_adamw(C.c_void_p(part.ctypes.data), len(part), args, stream)
+        records[:, field] = np.fromiter(map(_address, ts), dtype=np.uint64, count=len(ts))
+    if not params:
+        return
+    lib, stream = _lib.load(), raw_stream(device.index)
+    pairs = {(params[0].dtype, grads[0].dtype)} if one_kind else set(zip(map(_dtype, params), map(_dtype, grads)))
+    for pair in pairs:
+        part = records if one_kind else records[[(p.dtype, g.dtype) == pair for p, g in zip(params, grads)]]
+        args.p_dtype, args.g_dtype = _CODES[pair[0]], _CODES[pair[1]]
+        rc = lib.megray_adamw(C.c_void_p(part.__array_interface__["data"][0]), len(part), args, stream)
         if rc != 0:
             raise RuntimeError(f"megray_adamw failed ({rc})")

@@ -19,28 +19,33 @@ from .gemm import gemm_error_flag
 _CODES = {torch.float16: 6, torch.bfloat16: 10}
 
 
-def _tensor(t: torch.Tensor, shape, like: torch.Tensor, name: str):
+def _tensor(t, rows: int, heads: int, dim: int, dtype, index: int, name: str):
     """The C view of a [T, heads, D] tensor; ValueError for anything that the kernels do not read."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
-        raise ValueError(f"attention: {name} is a {tuple(shape)} {like.dtype} tensor on the queries' device")
-    rows, heads, dim = shape
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != index or
+            t.shape != (rows, heads, dim)):
+        raise ValueError(f"attention: {name} is a {(rows, heads, dim)} {dtype} tensor on the queries' device")
+    row, head, one = t.stride()
+    p = t.data_ptr()
     # the stride of an axis of one is never used
-    head = t.stride(1) if heads > 1 else dim
-    row = t.stride(0) if rows > 1 else max(8, heads * head)
-    if rows and (t.stride(2) != 1 or row % 8 or head % 8 or row <= 0 or head <= 0 or t.data_ptr() % 16):
+    if heads == 1:
+        head = dim
+    if rows <= 1:
+        row = max(8, heads * head)
+        if rows == 0:
+            return _lib.AttnTensor(p or None, row, dim)
+    if one != 1 or (row | head) & 7 or row <= 0 or head <= 0 or p & 15:
         raise ValueError(f"attention: {name}: innermost axis contiguous, the other strides multiples of 8 elements, "
                          "16-byte aligned")
-    return _lib.AttnTensor(t.data_ptr() or None, row, head)
+    return _lib.AttnTensor(p, row, head)
 
 
-def _output(t, shape, like: torch.Tensor, name: str):
-    t = torch.empty(shape, dtype=like.dtype, device=like.device) if t is None else t
-    c = _tensor(t, shape, like, name)
-    rows, heads, dim = shape
-    # (token by token or head by head, every element has an address of its own)
-    if rows > 1 and heads > 1 and not (c.head >= dim and c.row >= heads * c.head - (c.head - dim) or
-                                       c.row >= dim and c.head >= rows * c.row - (c.row - dim)) or \
-            (rows > 1 and c.row < dim):
+def _output(t, rows: int, heads: int, dim: int, like: torch.Tensor, index: int, partly: bool, name: str):
+    if t is None:  # what no prompt covers is zero
+        t = like.new_zeros(rows, heads, dim) if partly else like.new_empty(rows, heads, dim)
+    c = _tensor(t, rows, heads, dim, like.dtype, index, name)
+    # token by token or head by head, every element has an address of its own
+    if rows > 1 and not (c.head >= dim and c.row >= (heads - 1) * c.head + dim or
+                         c.row >= dim and c.head >= (rows - 1) * c.row + dim):
         raise ValueError(f"attention: {name} overlaps itself")
     return t, c
 
@@ -48,32 +53,32 @@ def _output(t, shape, like: torch.Tensor, name: str):
 def _problem(q, k, v, cu_seqlens, causal, scale):
     if not isinstance(q, torch.Tensor) or q.dim() != 3 or not q.is_cuda or q.dtype not in _CODES:
         raise ValueError("attention: q is a [T, heads, D] CUDA tensor, bf16 or float16")
-    tokens, heads, dim = q.shape
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise ValueError("attention: k is a [T, kv heads, D] tensor")
-    kv_heads = k.shape[1]
-    if dim % 8 or not 8 <= dim <= 128 or kv_heads < 1 or heads < 1 or heads % kv_heads:
+    tokens, heads, dim = q.shape
+    kv_heads, dtype, index = k.shape[1], q.dtype, q.get_device()
+    if dim & 7 or not 8 <= dim <= 128 or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("attention: D is a multiple of 8 from 8 to 128, the query heads a multiple of the key heads")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
-    if not 0.0 < scale < math.inf:
+    elif not 0.0 < scale < math.inf:
         raise ValueError("attention: scale is positive")
     cu, seqs = None, 1
     if cu_seqlens is not None:
-        if (cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or
-                not cu_seqlens.is_contiguous() or cu_seqlens.device != q.device):
+        if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or
+                not cu_seqlens.is_contiguous() or cu_seqlens.get_device() != index):
             raise ValueError("attention: cu_seqlens is a contiguous int32 tensor of at least 2 entries on q's device")
         cu, seqs = cu_seqlens.data_ptr(), cu_seqlens.numel() - 1
-    args = _lib.AttnArgs(cu, _CODES[q.dtype], tokens, heads, kv_heads, dim, seqs, int(bool(causal)), scale,
+    args = _lib.AttnArgs(cu, _CODES[dtype], tokens, heads, kv_heads, dim, seqs, 1 if causal else 0, scale,
                          gemm_error_flag(q.device).data_ptr())
-    kv = (tokens, kv_heads, dim)
-    return args, _tensor(q, q.shape, q, "q"), _tensor(k, kv, q, "k"), _tensor(v, kv, q, "v")
+    return (args, _tensor(q, tokens, heads, dim, dtype, index, "q"), _tensor(k, tokens, kv_heads, dim, dtype, index, "k"),
+            _tensor(v, tokens, kv_heads, dim, dtype, index, "v"), index)
 
 
-def _row_sums(t, heads: int, tokens: int, like: torch.Tensor, name: str) -> torch.Tensor:
+def _row_sums(t, heads: int, tokens: int, like: torch.Tensor, index: int, name: str) -> torch.Tensor:
     if t is None:
-        return torch.empty(heads, tokens, dtype=torch.float32, device=like.device)
-    if t.dtype != torch.float32 or t.shape != (heads, tokens) or not t.is_contiguous() or t.device != like.device:
+        return like.new_empty(heads, tokens, dtype=torch.float32)
+    if t.dtype is not torch.float32 or t.shape != (heads, tokens) or not t.is_contiguous() or t.get_device() != index:
         raise ValueError(f"attention: {name} is a contiguous [heads, T] float32 tensor on the queries' device")
     return t
 
@@ -85,18 +90,21 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     over several sets of keys are joined.  ``scale`` defaults to 1 / sqrt(D).
 
     Without ``cu_seqlens`` all rows are one prompt.  Rows behind the last prompt are not looked at and keep what
-    ``out`` and ``lse`` hold there (undefined in tensors made here).  ``cu_seqlens`` is read on the device: it has to
+    ``out`` and ``lse`` hold there (zeros in tensors made here).  ``cu_seqlens`` is read on the device: it has to
     rise from 0 to at most T; nothing outside the tensors is touched if it does not, but rows may then go
     unwritten.  Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32.  A NaN or
     an infinity in the values of a prompt may reach any row of that prompt, those of other prompts and of rows
     behind the last never do."""
-    if isinstance(q, torch.Tensor) and q.is_cuda and q.device.index != torch.cuda.current_device():
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention(q, k, v, cu_seqlens, causal=causal, scale=scale, out=out, lse=lse)
-    args, cq, ck, cv = _problem(q, k, v, cu_seqlens, causal, scale)
-    out, co = _output(out, q.shape, q, "out")
-    lse = _row_sums(lse, q.shape[1], q.shape[0], q, "lse")
-    rc = _lib.load().megray_attention(args, cq, ck, cv, co, lse.data_ptr(), raw_stream())
+    args, cq, ck, cv, index = _problem(q, k, v, cu_seqlens, causal, scale)
+    partly = cu_seqlens is not None
+    out, co = _output(out, args.tokens, args.heads, args.dim, q, index, partly, "out")
+    if lse is None and partly:
+        lse = q.new_zeros(args.heads, args.tokens, dtype=torch.float32)
+    lse = _row_sums(lse, args.heads, args.tokens, q, index, "lse")
+    rc = _lib.load().megray_attention(args, cq, ck, cv, co, lse.data_ptr(), raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"megray_attention failed ({rc})")
     return out, lse
@@ -108,22 +116,23 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     """Returns (dq, dk, dv) for the gradient ``dout`` of the ``out`` that :func:`attention` returned with ``lse`` for the
     same arguments.  Gradients of key / value heads are summed over the query heads that read them.  Given tensors
     are written to (any of the strides that the inputs may have, slices of one buffer among them); rows behind the
-    last prompt are left as they are.  No atomics: the same inputs give the same bits."""
-    if isinstance(q, torch.Tensor) and q.is_cuda and q.device.index != torch.cuda.current_device():
+    last prompt are left as they are (zeros in tensors made here).  No atomics: the same inputs give the same bits."""
+    if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention_bwd(dout, q, k, v, out, lse, cu_seqlens, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)
-    args, cq, ck, cv = _problem(q, k, v, cu_seqlens, causal, scale)
-    tokens, heads, _ = q.shape
-    co, cd = _tensor(out, q.shape, q, "out"), _tensor(dout, q.shape, q, "dout")
+    args, cq, ck, cv, index = _problem(q, k, v, cu_seqlens, causal, scale)
+    tokens, heads, kv_heads, dim, dtype = args.tokens, args.heads, args.kv_heads, args.dim, q.dtype
+    co = _tensor(out, tokens, heads, dim, dtype, index, "out")
+    cd = _tensor(dout, tokens, heads, dim, dtype, index, "dout")
     if lse is None:
         raise ValueError("attention_bwd: lse is what attention returned")
-    lse = _row_sums(lse, heads, tokens, q, "lse")
-    dq, cdq = _output(dq, q.shape, q, "dq")
-    dk, cdk = _output(dk, k.shape, q, "dk")
-    dv, cdv = _output(dv, k.shape, q, "dv")
-    delta = torch.empty(heads, tokens, dtype=torch.float32, device=q.device)
+    lse = _row_sums(lse, heads, tokens, q, index, "lse")
+    dq, cdq = _output(dq, tokens, heads, dim, q, index, cu_seqlens is not None, "dq")
+    dk, cdk = _output(dk, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dk")
+    dv, cdv = _output(dv, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dv")
+    delta = q.new_empty(heads, tokens, dtype=torch.float32)
     rc = _lib.load().megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, delta.data_ptr(),
-                                          raw_stream())
+                                          raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"megray_attention_bwd failed ({rc})")
     return dq, dk, dv

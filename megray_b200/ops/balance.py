@@ -13,38 +13,42 @@ _CODES = {torch.float32: 7, torch.bfloat16: 10}
 def _router(logits: torch.Tensor, idx: torch.Tensor, mask):
     if logits.dim() != 2 or logits.dtype not in _CODES or not logits.is_cuda or logits.stride(1) != 1:
         raise ValueError("balance: logits is a [tokens, experts] CUDA tensor, float32 or bf16, with contiguous rows")
-    tokens, experts = logits.shape
+    (tokens, experts), index = logits.shape, logits.get_device()
     if not 1 <= experts <= 1024:
         raise ValueError("balance: 1 to 1024 experts")
-    if (idx.dim() != 2 or idx.shape[0] != tokens or not 1 <= idx.shape[1] <= 64 or idx.device != logits.device or
+    if (idx.dim() != 2 or idx.shape[0] != tokens or not 1 <= idx.shape[1] <= 64 or idx.get_device() != index or
             idx.dtype not in (torch.int32, torch.int64) or not idx.is_contiguous()):
         raise ValueError("balance: idx is a contiguous [tokens, 1..64] int32 or int64 tensor on the logits' device")
-    if tokens * idx.shape[1] >= 2 ** 31:
+    top = idx.shape[1]
+    if tokens * top >= 2 ** 31:
         raise ValueError("balance: fewer than 2^31 pairs")
     if mask is not None and (mask.shape != (tokens,) or mask.dtype not in (torch.bool, torch.uint8) or
-                             mask.device != logits.device or not mask.is_contiguous()):
+                             mask.get_device() != index or not mask.is_contiguous()):
         raise ValueError("balance: mask is a contiguous [tokens] bool or uint8 tensor on the logits' device")
     ld = logits.stride(0) if tokens > 1 else experts
     if ld < experts:
         raise ValueError("balance: rows of the logits overlap")
-    return _lib.Router(logits.data_ptr(), idx.data_ptr(), mask.data_ptr() if mask is not None else None, ld,
-                       _CODES[logits.dtype], int(idx.dtype == torch.int64), tokens, experts, idx.shape[1])
+    return _lib.Router(logits.data_ptr(), idx.data_ptr(), None if mask is None else mask.data_ptr(), ld,
+                       _CODES[logits.dtype], 1 if idx.dtype is torch.int64 else 0, tokens, experts, top), index
 
 
-def _out(logits: torch.Tensor, coef: float, dlogits, accumulate: bool):
-    tokens, experts = logits.shape
+def _out(logits: torch.Tensor, tokens: int, experts: int, index: int, coef: float, dlogits, accumulate: bool):
+    ldd = experts
     if dlogits is None:
         if accumulate:
             raise ValueError("balance: accumulate adds to dlogits, which is not given")
-        dlogits = torch.empty(tokens, experts, dtype=logits.dtype, device=logits.device)
-    if (dlogits.shape != logits.shape or dlogits.device != logits.device or
-            dlogits.dtype not in (logits.dtype, torch.float32) or (dlogits.numel() and dlogits.stride(1) != 1) or
-            (tokens > 1 and dlogits.stride(0) < experts)):
-        raise ValueError("balance: dlogits has the logits' shape and device, their type or float32, and contiguous rows")
-    loss = torch.empty(1, dtype=torch.float32, device=logits.device)
-    counts = torch.empty(experts, dtype=torch.int32, device=logits.device)
-    out = _lib.BalanceOut(loss.data_ptr(), counts.data_ptr(), dlogits.data_ptr() or None,
-                          dlogits.stride(0) if tokens > 1 else experts, _CODES[dlogits.dtype], int(accumulate), coef)
+        dlogits = logits.new_empty(tokens, experts)
+    else:
+        if (dlogits.shape != (tokens, experts) or dlogits.get_device() != index or
+                dlogits.dtype not in (logits.dtype, torch.float32) or (dlogits.numel() and dlogits.stride(1) != 1) or
+                (tokens > 1 and dlogits.stride(0) < experts)):
+            raise ValueError("balance: dlogits has the logits' shape and device, their type or float32, and contiguous rows")
+        if tokens > 1:
+            ldd = dlogits.stride(0)
+    loss = logits.new_empty(1, dtype=torch.float32)
+    counts = logits.new_empty(experts, dtype=torch.int32)
+    out = _lib.BalanceOut(loss.data_ptr(), counts.data_ptr(), dlogits.data_ptr() or None, ldd, _CODES[dlogits.dtype],
+                          1 if accumulate else 0, coef)
     return out, loss, counts, dlogits
 
 
@@ -66,14 +70,14 @@ def balance_loss_grad(logits: torch.Tensor, idx: torch.Tensor, coef: float, *, m
 
     With ``comm`` (a communicator of several ranks; a collective call) counts, means and Tv are taken over the tokens
     of all ranks, and ``dlogits`` is the gradient of that one loss with respect to this rank's logits."""
-    if logits.is_cuda and logits.device.index != torch.cuda.current_device():
+    if logits.is_cuda and logits.get_device() != torch.cuda.current_device():
         with torch.cuda.device(logits.device):
             return balance_loss_grad(logits, idx, coef, mask=mask, dlogits=dlogits, accumulate=accumulate, comm=comm)
-    router = _router(logits, idx, mask)
-    out, loss, counts, dlogits = _out(logits, coef, dlogits, accumulate)
-    lib, stream = _lib.load(), raw_stream()
-    tokens, experts = logits.shape
-    room = torch.empty(lib.megray_balance_workspace(tokens, experts), dtype=torch.uint8, device=logits.device)
+    router, index = _router(logits, idx, mask)
+    tokens, experts = router.tokens, router.experts
+    out, loss, counts, dlogits = _out(logits, tokens, experts, index, coef, dlogits, accumulate)
+    lib, stream = _lib.load(), raw_stream(index)
+    room = logits.new_empty(lib.megray_balance_workspace(tokens, experts), dtype=torch.uint8)
     if comm is None or comm.nranks == 1:
         rc = lib.megray_balance(router, out, room.data_ptr(), stream)
         if rc != 0:

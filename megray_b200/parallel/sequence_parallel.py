@@ -15,14 +15,18 @@ NVL or NCCL backend, CPU tensors on the host backend, which is how the tests run
   (maximum, denominator, weighted sum in fp32) absorbs one block per step.  With ``causal=True``
   blocks that lie entirely in the future are skipped and the diagonal block is masked.
 
-The attention arithmetic itself is plain torch; what this module contributes is the
-communication schedule.
+The attention arithmetic of these is plain torch, for tensors of any device and type; what this module
+contributes is the communication schedule.  ``ulysses_attention_packed`` and its backward pass run the same swap
+around the library's attention kernels: prompts packed one behind the other, grouped key / value heads,
+16-bit CUDA tensors.
 """
 from __future__ import annotations
 
 import math
 
 import torch
+
+from ..ops.attention import attention, attention_bwd
 
 
 # ---------------------------------------------------------------------------------- Ulysses
@@ -66,6 +70,24 @@ def ulysses_attention(comm, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, c
     qh, kh, vh = (seq_to_heads(comm, t) for t in (q, k, v))
     out = _attention(qh, kh, vh, causal, 0, 0)
     return heads_to_seq(comm, out.to(q.dtype))
+
+
+def ulysses_attention_packed(comm, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor = None,
+                             *, causal: bool = True, scale: float = None):
+    """Attention over packed prompts for row-sharded ``[T/n, H, D]`` queries and ``[T/n, Hk, D]`` keys and values: swap
+    to head shards, :func:`megray_b200.ops.attention` over all T rows, swap back.  H and Hk are divisible by the number
+    of ranks; ``cu_seqlens`` counts rows of the whole batch and is the same on every rank.  Returns (out, saved); ``saved``
+    goes to :func:`ulysses_attention_packed_bwd`.  Rows behind the last prompt are zero."""
+    qh, kh, vh = (seq_to_heads(comm, t) for t in (q, k, v))
+    out, lse = attention(qh, kh, vh, cu_seqlens, causal=causal, scale=scale)
+    return heads_to_seq(comm, out), (qh, kh, vh, out, lse, cu_seqlens, causal, scale)
+
+
+def ulysses_attention_packed_bwd(comm, dout: torch.Tensor, saved):
+    """(dq, dk, dv) of this rank's rows for the gradient of its rows of :func:`ulysses_attention_packed`'s result."""
+    qh, kh, vh, out, lse, cu_seqlens, causal, scale = saved
+    grads = attention_bwd(seq_to_heads(comm, dout), qh, kh, vh, out, lse, cu_seqlens, causal=causal, scale=scale)
+    return tuple(heads_to_seq(comm, g) for g in grads)
 
 
 # ---------------------------------------------------------------------------------- ring attention

@@ -25,6 +25,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "f32x2.cuh"
 #include "gemm_device.cuh"
 #include "launch_count.h"
@@ -1251,11 +1253,26 @@ cudaError_t pick(const Problem& p, F go) {
         return p.fp16 ? go(std::integral_constant<int, 64>{}, T{}) : go(std::integral_constant<int, 64>{}, N{});
     return p.fp16 ? go(std::integral_constant<int, 128>{}, T{}) : go(std::integral_constant<int, 128>{}, N{});
 }
-// (the attribute belongs to a function on a device: it is set before every launch, which costs under a microsecond)
+// Lets `kernel` have its shared memory on the current device, once for each
+template <class... P>
+cudaError_t allow_smem(void (*kernel)(P...), std::atomic<uint64_t>& done, int smem) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess)
+        return e;
+    const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+    if (done.load(std::memory_order_acquire) & bit)
+        return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+        done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
 // `early`: the kernel may start before the one in front of it has ended
-template <class... P, class... A>
-cudaError_t run(void (*kernel)(P...), unsigned grid, int threads, int smem, bool early, cudaStream_t stream, const A&... args) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto KERNEL, class... A>
+cudaError_t run(unsigned grid, int threads, int smem, bool early, cudaStream_t stream, const A&... args) {
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_smem(KERNEL, done, smem);
     if (e != cudaSuccess)
         return e;
     cudaLaunchAttribute attr{};
@@ -1268,7 +1285,7 @@ cudaError_t run(void (*kernel)(P...), unsigned grid, int threads, int smem, bool
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = early ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    e = cudaLaunchKernelEx(&cfg, KERNEL, args...);
     count_launch();
     return e;
 }
@@ -1293,7 +1310,7 @@ cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tenso
     a.lse = lse;
     return pick(p, [&](auto dp, auto half) {
         constexpr int DP = decltype(dp)::value;
-        return run(forward_kernel<DP, decltype(half)::value>, grid, FWD_THREADS, fwd_smem<DP>(), false, stream, mq, mk, mv, a);
+        return run<forward_kernel<DP, decltype(half)::value>>(grid, FWD_THREADS, fwd_smem<DP>(), false, stream, mq, mk, mv, a);
     });
 }
 
@@ -1334,13 +1351,13 @@ cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, T
         a.out1 = static_cast<uint16_t*>(dv.p);
         a.row1 = dv.row;
         a.head1 = dv.head;
-        const cudaError_t first = run(dkv_kernel<DP, FP16>, grid_k, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
+        const cudaError_t first = run<dkv_kernel<DP, FP16>>(grid_k, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
         if (first != cudaSuccess)
             return first;
         a.out0 = static_cast<uint16_t*>(dq.p);
         a.row0 = dq.row;
         a.head0 = dq.head;
-        return run(dq_kernel<DP, FP16>, grid_q, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
+        return run<dq_kernel<DP, FP16>>(grid_q, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
     });
 }
 
