@@ -18,8 +18,8 @@
 // Bound by HBM, with the issue slots close behind: 10 bytes an element with 8-bit moments and bf16 tensors leave
 // about 55 instructions for it; products and sums are issued in pairs.  A warp takes blocks of 256 elements, two
 // runs of four a lane so that every access of the warp is contiguous whatever the types, and loads the next block
-// before it works on one (latency, not bandwidth, was the limit without: 40 M elements 97 us).  A scale is found with
-// one warp-wide integer maximum (float magnitudes order as integers, NaN above all) and nothing is read twice.
+// before it works on one (without: 550 us for 176 M elements at four CTAs an SM, 430 with).  A scale is found with one
+// warp-wide integer maximum (float magnitudes order as integers, NaN above all) and nothing is read twice.
 // Tensors' addresses travel as kernel parameters: no copy to the device before the launch, and a captured
 // graph replays them.
 #include "adamw.cuh"
@@ -57,7 +57,7 @@ struct Table {
     Entry e[CAP];
     uint32_t first_cta[CAP];
     int count;
-    int per_warp;  // blocks that a warp takes, kWarps apart
+    int per_warp;  // neighbouring blocks that a warp takes, 32 at most
 };
 
 struct Args {
@@ -228,7 +228,6 @@ template <class P, class G, int BITS>
 struct Raw {
     static constexpr int MW = BITS == 8 ? 2 : 8;
     uint32_t p[words_of<P>()], g[words_of<G>()], m[MW], v[MW];
-    float sm, sv;
 };
 
 template <class P, class G, int BITS, int CAP>
@@ -285,8 +284,6 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? 4 : 3) adamw_kernel(cons
                 r.m[h] = __ldcs(reinterpret_cast<const uint32_t*>(m0 + at + 128 * h));
                 r.v[h] = __ldcs(reinterpret_cast<const uint32_t*>(v0 + at + 128 * h));
             }
-            r.sm = a.m_scale[sb0 + block];
-            r.sv = a.v_scale[sb0 + block];
         } else {
             load_words(m0 + at, true, 0, r.m);
             load_words(v0 + at, true, 0, r.v);
@@ -294,26 +291,33 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? 4 : 3) adamw_kernel(cons
     };
 
     Raw<P, G, BITS> raw;
-    const int first = threadIdx.x >> 5;
-    if (first * kBlock < n)
+    const int first = (threadIdx.x >> 5) * t.per_warp, past = min(first + t.per_warp, (n + kBlock - 1) / kBlock);
+    float scales[2] = {0.f, 0.f}, new_scales[2] = {0.f, 0.f};  // of block first + lane
+    if (BITS == 8 && first + lane < past) {
+        scales[0] = a.m_scale[sb0 + first + lane];
+        scales[1] = a.v_scale[sb0 + first + lane];
+    }
+    if (first < past)
         load(first, raw);
 #pragma unroll 1
-    for (int block = first; block * kBlock < n; block += kWarps) {
+    for (int block = first; block < past; ++block) {
         float p[8], g[8], m[8], v[8];
         unpack<P>(raw.p, p);
         unpack<G>(raw.g, g);
         if constexpr (BITS == 8) {
+            const float sm = __shfl_sync(0xffffffffu, scales[0], block - first);
+            const float sv = __shfl_sync(0xffffffffu, scales[1], block - first);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                decode4(raw.m[h], raw.sm, m + 4 * h);
-                decode4(raw.v[h], raw.sv, v + 4 * h);
+                decode4(raw.m[h], sm, m + 4 * h);
+                decode4(raw.v[h], sv, v + 4 * h);
             }
         } else {
             unpack<float>(raw.m, m);
             unpack<float>(raw.v, v);
         }
-        if ((block + kWarps) * kBlock < n)
-            load(block + kWarps, raw);
+        if (block + 1 < past)
+            load(block + 1, raw);
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
             Pair mm{m[i], m[i + 1]}, vv{v[i], v[i + 1]};
@@ -352,14 +356,18 @@ __global__ void __launch_bounds__(kThreads, BITS == 8 ? 4 : 3) adamw_kernel(cons
             to = reinterpret_cast<uint32_t*>(v0 + at);
             to[0] = code[0];
             to[32] = code[1];
-            if (lane == 0) {
-                a.m_scale[sb0 + block] = sm;
-                a.v_scale[sb0 + block] = sv;
+            if (lane == block - first) {
+                new_scales[0] = sm;
+                new_scales[1] = sv;
             }
         } else {
             store_some(m0 + at, true, 0, m);
             store_some(v0 + at, true, 0, v);
         }
+    }
+    if (BITS == 8 && first + lane < past) {
+        a.m_scale[sb0 + first + lane] = new_scales[0];
+        a.v_scale[sb0 + first + lane] = new_scales[1];
     }
 }
 
@@ -369,9 +377,12 @@ cudaError_t launch_table(const Tensor* tensors, int count, const Args& a, cudaSt
     uint64_t blocks = 0;
     for (int k = 0; k < count; ++k)
         blocks += (tensors[k].n + kBlock - 1) / kBlock;
-    // four blocks a warp once that still fills the chip three times over (what a warp does once, finding its
-    // tensor above all, costs as many instructions as a block), else one, for the shortest way through
-    t.per_warp = blocks >= 148ull * 3 * kWarps * 12 ? 4 : 1;
+    // Several blocks a warp once that still fills the chip (what a warp does once, finding its tensor above all, costs
+    // as many instructions as a block), eight of 8-bit moments, whose scales then are one whole sector to read and
+    // to write: written one by one they held everything else up (176 M elements: 430 us, 297 so; at 4 a warp 310).
+    // With 32 bits eight are 3 % slower than four.
+    const uint64_t resident = 148ull * 4 * kWarps;
+    t.per_warp = BITS == 8 && blocks >= resident * 8 * 4 ? 8 : blocks >= resident * 4 * 3 ? 4 : 1;
     const uint64_t chunk = static_cast<uint64_t>(kBlock) * kWarps * t.per_warp;
     int i = 0;
     while (i < count) {
