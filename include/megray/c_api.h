@@ -185,7 +185,7 @@ int megray_rmsnorm_bwd_bf16(const void* dn, const void* n, const float* inv_rms,
 /* Softmax attention over prompts that are packed one behind the other (src/kernels/attention.cuh).  Tensors are [tokens,
  * heads, dim] with strides in elements, multiples of 8, the innermost contiguous, 16-byte aligned.  Sequence s holds rows
  * cu[s] .. cu[s + 1] (device array of seqs + 1); without cu all rows are one.  Rows behind the last sequence are neither
- * used nor written.  lse is [heads, tokens]; `delta` a workspace of heads * tokens floats. */
+ * used nor written.  lse is [heads, tokens]; `workspace` holds megray_attention_bwd_workspace(args) bytes, 16-byte aligned. */
 typedef struct {
     void* p;
     int64_t row, head;
@@ -202,7 +202,8 @@ int megray_attention(const megray_attn_args* a, const megray_attn_tensor* q, con
 int megray_attention_bwd(const megray_attn_args* a, const megray_attn_tensor* dout, const megray_attn_tensor* q,
                          const megray_attn_tensor* k, const megray_attn_tensor* v, const megray_attn_tensor* out,
                          const float* lse, const megray_attn_tensor* dq, const megray_attn_tensor* dk,
-                         const megray_attn_tensor* dv, float* delta, void* stream);
+                         const megray_attn_tensor* dv, void* workspace, void* stream);
+size_t megray_attention_bwd_workspace(const megray_attn_args* a);  /* 0 for arguments that are refused */
 
 /* AdamW over a list of tensors.  `block` is the tensor's first block of 256 elements in the moment buffers,
  * which cover whole blocks.  bits = 32: m and v are float32; bits = 8: m and v hold e4m3 numbers of m and of

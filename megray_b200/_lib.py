@@ -193,6 +193,7 @@ def _declare(lib) -> None:
     at = P(AttnTensor)
     d("megray_attention", i32, P(AttnArgs), at, at, at, at, vp, vp)
     d("megray_attention_bwd", i32, P(AttnArgs), at, at, at, at, at, vp, at, at, at, vp, vp)
+    d("megray_attention_bwd_workspace", sz, P(AttnArgs))
     d("megray_adamw", i32, vp, i32, P(AdamWArgs), vp)
     d("megray_balance_workspace", sz, i32, i32)
     d("megray_balance_partials", i32, i32, i32)

@@ -130,9 +130,9 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     dq, cdq = _output(dq, tokens, heads, dim, q, index, cu_seqlens is not None, "dq")
     dk, cdk = _output(dk, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dk")
     dv, cdv = _output(dv, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dv")
-    delta = q.new_empty(heads, tokens, dtype=torch.float32)
-    rc = _lib.load().megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, delta.data_ptr(),
-                                          raw_stream(index))
+    lib = _lib.load()
+    room = q.new_empty(lib.megray_attention_bwd_workspace(args), dtype=torch.uint8)
+    rc = lib.megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, room.data_ptr(), raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"megray_attention_bwd failed ({rc})")
     return dq, dk, dv

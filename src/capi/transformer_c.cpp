@@ -45,14 +45,18 @@ int megray_attention(const megray_attn_args* a, const megray_attn_tensor* q, con
         return kInvalid;
     return rc(mgk::attn::launch_forward(p, T(q), T(k), T(v), T(out), lse, S(stream)));
 }
+size_t megray_attention_bwd_workspace(const megray_attn_args* a) {
+    mgk::attn::Problem p;
+    return to_problem(a, &p) ? mgk::attn::backward_workspace(p) : 0;
+}
 int megray_attention_bwd(const megray_attn_args* a, const megray_attn_tensor* dout, const megray_attn_tensor* q,
                          const megray_attn_tensor* k, const megray_attn_tensor* v, const megray_attn_tensor* out,
                          const float* lse, const megray_attn_tensor* dq, const megray_attn_tensor* dk,
-                         const megray_attn_tensor* dv, float* delta, void* stream) {
+                         const megray_attn_tensor* dv, void* workspace, void* stream) {
     mgk::attn::Problem p;
     if (!to_problem(a, &p))
         return kInvalid;
-    return rc(mgk::attn::launch_backward(p, T(dout), T(q), T(k), T(v), T(out), lse, T(dq), T(dk), T(dv), delta, S(stream)));
+    return rc(mgk::attn::launch_backward(p, T(dout), T(q), T(k), T(v), T(out), lse, T(dq), T(dk), T(dv), workspace, S(stream)));
 }
 
 int megray_adamw(const megray_adamw_tensor* tensors, int count, const megray_adamw_args* a, void* stream) {

@@ -55,6 +55,9 @@ struct Params {
     int64_t row0, head0, row1, head1;
     float* lse;
     const float* delta;
+    int tiles_per_cta;  // forward: tiles of queries
+    int splits;         // dK and dV: CTAs that share the queries of one tile of keys
+    float* part;        // their partial sums, [dK, dV][splits][tokens][kv_heads][dim], when splits > 1
 };
 
 // ---------------------------------------------------------------- PTX beyond ptx_sm100.cuh
@@ -332,6 +335,19 @@ __device__ __forceinline__ void store_row(uint32_t taddr, int from, int to, floa
     }
 }
 
+// The same as float32
+__device__ __forceinline__ void store_sums(uint32_t taddr, int from, int to, float* row, bool write) {
+    for (int c = from; c < to; c += 32) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(taddr + c, r);
+        tmem_ld_wait(r);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+            if (write && c + i < to)
+                *reinterpret_cast<uint4*>(row + c + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+    }
+}
+
 // ================================================================ forward
 //
 // A CTA takes two tiles of 128 queries of one head and walks over the keys once; while one warpgroup works on the
@@ -355,7 +371,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                        const __grid_constant__ CUtensorMap map_v, const Params p) {
     constexpr int TB = tile_bytes<DP>();
     // the last tiles of a sequence, which have the most keys, come first
-    auto first_row = [](const Where& w) { return (w.tiles - 1 - w.local) * 2 * TILE; };
+    const int rows = p.tiles_per_cta * TILE;
+    auto first_row = [&](const Where& w) { return (w.tiles - 1 - w.local) * rows; };
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align_1024(smem_raw);
     uint8_t* ring = smem + 2 * TB;
@@ -386,7 +403,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             mbar_fence_init();
             fence_proxy_async_smem();
         }
-        const Where found = find_tile(p, 2 * TILE, static_cast<int>(blockIdx.x / p.heads));
+        const Where found = find_tile(p, rows, static_cast<int>(blockIdx.x / p.heads));
         __syncwarp();
         if (elect_one()) {
             *where = found;
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                 const int first = first_row(found);
                 load_tile<DP>(smem_u32(smem), &map_q, q_full, head, found.start + first);
                 load_tile<DP>(smem_u32(ring), &map_k, full0, kv_head, found.start);
-                if (first + TILE < found.len)
+                if (rows > TILE && first + TILE < found.len)
                     load_tile<DP>(smem_u32(smem) + TB, &map_q, q_full + 8, head, found.start + first + TILE);
             }
         }
@@ -421,7 +438,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
     for (int t = 0; t < 2; ++t) {
         const int first = r0 + t * TILE;
         const int keys = p.causal ? min(w.len, first + TILE) : w.len;
-        n_blocks[t] = first < w.len ? (keys + TILE - 1) / TILE : 0;
+        n_blocks[t] = t < p.tiles_per_cta && first < w.len ? (keys + TILE - 1) / TILE : 0;
     }
     const int n = max(n_blocks[0], n_blocks[1]);
     WaitCtx wc{abort_flag, WAIT_NS};
@@ -906,6 +923,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 // score tiles are keys, so P^T and dS^T are left operands as they stand.
 // Scores and their gradients take turns in one region of TMEM, A; probabilities and score gradients as 16-bit operands
 // lie in another, B, so that neither waits for the product that reads the other:
+// Where there are few tiles of keys, several CTAs share the queries of one and leave float32 sums that a last kernel
+// adds up in order.
 //   tensor cores:  dV += P^T(i-1) dO, A = dP^T(i), dK += dS^T(i-1) Q, A = S^T(i+1), ...
 //   row warps:     P(i) from S(i) (in registers: A is free at once)    dS(i) from dP(i)
 // (P written over S and dS over dP, so that S(i+1) waited for dV: 3180 cycles an iteration; the products take 2048.)
@@ -933,7 +952,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int lane = threadIdx.x & 31;
-    const int kv_head = static_cast<int>(blockIdx.x % p.kv_heads);
+    const int split = static_cast<int>(blockIdx.x % p.splits), kv_head = static_cast<int>(blockIdx.x / p.splits % p.kv_heads);
     const int group = p.heads / p.kv_heads;
     if (warp == TMA_WARP) {
         if (lane == 0) {
@@ -956,7 +975,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             mbar_fence_init();
             fence_proxy_async_smem();
         }
-        const Where found = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.kv_heads));
+        const Where found = find_tile(p, TILE, static_cast<int>(blockIdx.x / p.splits / p.kv_heads));
         __syncwarp();
         if (elect_one()) {
             *where = found;
@@ -984,15 +1003,18 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     const int k0 = w.local * TILE;               // the first keys, which the most queries see, come first
     const int i0 = p.causal ? w.local : 0;       // first block of queries that sees them
     const int per_head = w.tiles - i0;
-    const int n = group * per_head;
+    // this CTA's share of the blocks of queries of all heads of the group
+    const int all = group * per_head;
+    const int first = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
+    const int n = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits) - first;
     WaitCtx wc{abort_flag, WAIT_NS};
 
     if (warp == TMA_WARP) {
         set_registers_down<64>();
         uint32_t side_phase = 0;
         for (int it = 0; it < n; ++it) {
-            const int s = it % LONG_STAGES, so = it % SHORT_STAGES, head = kv_head * group + it / per_head;
-            const int q0 = (i0 + it % per_head) * TILE;
+            const int s = it % LONG_STAGES, so = it % SHORT_STAGES, head = kv_head * group + (first + it) / per_head;
+            const int q0 = (i0 + (first + it) % per_head) * TILE;
             if (!__all_sync(0xffffffffu, mbar_wait(q_empty + 8 * s, ((it / LONG_STAGES) & 1) ^ 1, wc)) ||
                 !feed<DP>(ring_q + s * TB, &map_q, q_full + 8 * s, side, side_phase, head, w.start + q0, w.len - q0, wc))
                 break;
@@ -1007,7 +1029,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         next_kernel_may_start();
         // -lse log2 e and -delta of every block's rows; a row behind the end has probabilities of zero
         for (int it = 0; it < n; ++it) {
-            const int s = it % SHORT_STAGES, head = kv_head * group + it / per_head, q0 = (i0 + it % per_head) * TILE;
+            const int s = it % SHORT_STAGES, head = kv_head * group + (first + it) / per_head, q0 = (i0 + (first + it) % per_head) * TILE;
             if (!__all_sync(0xffffffffu, mbar_wait(st_empty + 8 * s, ((it / SHORT_STAGES) & 1) ^ 1, wc)))
                 break;
             float* to = stats + s * 2 * TILE;
@@ -1073,7 +1095,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
             };
             // barriers are asked ahead of the products before which they are needed, so that the answers come while
             // others are issued
-            bool ok = issue_wait(kv_full, 0, wc) && scores(0, false);
+            bool ok = issue_wait(kv_full, 0, wc) && n > 0 && scores(0, false);  // (the copies are waited for in any case)
             for (int it = 0; ok && it < n; ++it) {
                 const bool o_now = o_here(it);
                 if (it > 0)
@@ -1105,7 +1127,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         const float c = p.scale * LOG2E;
         bool ok = true;
         for (int it = 0; it < n; ++it) {
-            const int s = it % SHORT_STAGES, q0 = (i0 + it % per_head) * TILE + part * 32;
+            const int s = it % SHORT_STAGES, q0 = (i0 + (first + it) % per_head) * TILE + part * 32;
             const float4* minus_lse = reinterpret_cast<const float4*>(stats + s * 2 * TILE + part * 32);
             const float4* minus_delta = minus_lse + TILE / 4;
             float pr[32], dp[32];
@@ -1131,7 +1153,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 pr[e + 2] = b.x;
                 pr[e + 3] = b.y;
             }
-            if (p.causal && it % per_head == 0) {
+            if (p.causal && (first + it) % per_head == 0) {
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
                     if (q0 + e < key)
@@ -1175,12 +1197,20 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                 mbar_arrive(ds_ready);
             }
         }
-        if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, wc))) {
+        const bool live = key < w.len;
+        const int64_t at = w.start + static_cast<int64_t>(key);
+        const int from = (part & 1) * (DP / 2), to = (part & 1) ? p.dim : min(p.dim, DP / 2);
+        float* sums = p.part + (((part < 2 ? 0 : p.splits) + split) * static_cast<int64_t>(p.tokens) + at) * p.kv_heads * p.dim +
+                      kv_head * p.dim;
+        if (n == 0) {  // (only where there are more CTAs than blocks of queries)
+            if (live)
+                for (int c = from; c < to; c += 4)
+                    *reinterpret_cast<float4*>(sums + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (ok && __all_sync(0xffffffffu, mbar_wait(done, 0, wc))) {
             tc_fence_after();
-            const bool live = key < w.len;
-            const int64_t at = w.start + static_cast<int64_t>(key);
-            const int from = (part & 1) * (DP / 2), to = (part & 1) ? p.dim : min(p.dim, DP / 2);
-            if (part < 2)
+            if (p.splits > 1)
+                store_sums((part < 2 ? t_dk : t_dv) + lanes, from, to, sums, live);
+            else if (part < 2)
                 store_row<FP16>(t_dk + lanes, from, to, p.scale, p.out0 + at * p.row0 + kv_head * p.head0, live);
             else
                 store_row<FP16>(t_dv + lanes, from, to, 1.f, p.out1 + at * p.row1 + kv_head * p.head1, live);
@@ -1195,6 +1225,36 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         tmem_dealloc_cg1(tmem, 512);
     if (threadIdx.x == 0 && *abort_flag && p.error_flag != nullptr)
         *p.error_flag = 1;
+}
+
+// Sums of the splits in their order, rounded once: dK (times scale) and dV of the rows that sequences cover.  A thread
+// takes eight elements.  Bound by reading the partial sums.
+template <bool FP16>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+    const int pieces = p.dim / 8;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, one = static_cast<int64_t>(p.tokens) * p.kv_heads * pieces;
+    if (i >= 2 * one)
+        return;
+    const int which = i >= one ? 1 : 0;
+    const int64_t j = i - which * one, at = j / (p.kv_heads * pieces);
+    const int kv_head = static_cast<int>(j / pieces % p.kv_heads), c = static_cast<int>(j % pieces) * 8;
+    if (p.cu != nullptr && (at < p.cu[0] || at >= p.cu[p.seqs]))
+        return;
+    const float* sums = p.part + (which * p.splits * static_cast<int64_t>(p.tokens) + at) * p.kv_heads * p.dim + kv_head * p.dim + c;
+    float v[8] = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const float4 a = __ldcs(reinterpret_cast<const float4*>(sums)), b = __ldcs(reinterpret_cast<const float4*>(sums) + 1);
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+        sums += static_cast<int64_t>(p.tokens) * p.kv_heads * p.dim;
+    }
+    const float f = which ? 1.f : p.scale;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        w[k] = pack2<FP16>(v[2 * k] * f, v[2 * k + 1] * f);
+    uint16_t* to = which ? p.out1 + at * p.row1 + kv_head * p.head1 : p.out0 + at * p.row0 + kv_head * p.head0;
+    *reinterpret_cast<uint4*>(to + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // ================================================================ host side
@@ -1299,11 +1359,15 @@ cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tenso
         return cudaSuccess;
     if (bad(q) || bad(k) || bad(v) || bad(out) || lse == nullptr || (reinterpret_cast<uintptr_t>(lse) & 3))
         return cudaErrorInvalidValue;
-    const unsigned grid = grid_for(p, 2 * TILE, p.heads);
+    // Two tiles a CTA while that makes a CTA for every processor, else one: a tile alone takes as long as two, which
+    // work in turns.  (1000 tokens, 8 heads of 64: 14.8 us with one, 16.9 with two; 16384 tokens, 8 heads: 753 and 437.)
+    const int tiles = grid_for(p, 2 * TILE, p.heads) >= 148 ? 2 : 1;
+    const unsigned grid = grid_for(p, tiles * TILE, p.heads);
     CUtensorMap mq, mk, mv;
     if (grid == 0 || !make_map(&mq, q, p.heads, p) || !make_map(&mk, k, p.kv_heads, p) || !make_map(&mv, v, p.kv_heads, p))
         return cudaErrorInvalidValue;
     Params a = params(p);
+    a.tiles_per_cta = tiles;
     a.out0 = static_cast<uint16_t*>(out.p);
     a.row0 = out.row;
     a.head0 = out.head;
@@ -1314,19 +1378,45 @@ cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tenso
     });
 }
 
+// CTAs that share one tile of keys.  A tile takes the heads of its group one after the other, so that with grouped heads
+// few tiles mean long ones: then about two CTAs a processor, but no more than the group has heads (dQ runs beside and
+// has as long to go for one head).  4096 tokens, 4 heads of one group: 198 us unshared, 114 by two, 99 by ten; 2048
+// tokens, 16 heads in 2 groups: 203, 118 and 88.  Without groups sharing only costs (1000 tokens, 8 heads: 17 us
+// unshared, 25 by two), and so it does where there is a CTA for every processor (5003 tokens, 12 heads in 4 groups: 137
+// and 160).
+static int splits_for(const Problem& p) {
+    const int64_t seqs = p.cu != nullptr ? p.seqs : 1, group = p.heads / p.kv_heads;
+    // (where the sequences end is not known here: half a tile is taken to be empty in each)
+    const int64_t full = (p.tokens + TILE - 1) / TILE, ctas = ((full > seqs ? full : seqs) + seqs / 2) * p.kv_heads;
+    if (ctas >= 148 || p.tokens == 0)
+        return 1;
+    const int64_t want = (296 + ctas - 1) / ctas, most = group < 16 ? group : 16;
+    return static_cast<int>(want < most ? want : most);
+}
+
+size_t backward_workspace(const Problem& p) {
+    if (bad(p))
+        return 0;
+    const size_t rows = static_cast<size_t>(p.tokens) * p.heads, splits = splits_for(p);
+    const size_t part = splits > 1 ? 2 * splits * p.tokens * p.kv_heads * p.dim : 0;
+    return ((rows + 3) / 4 * 4 + part) * sizeof(float);
+}
+
 cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, const float* lse,
-                            Tensor dq, Tensor dk, Tensor dv, float* delta, cudaStream_t stream) {
+                            Tensor dq, Tensor dk, Tensor dv, void* workspace, cudaStream_t stream) {
     if (bad(p))
         return cudaErrorInvalidValue;
     if (p.tokens == 0)
         return cudaSuccess;
-    if (bad(dout) || bad(q) || bad(k) || bad(v) || bad(out) || bad(dq) || bad(dk) || bad(dv) || lse == nullptr || delta == nullptr ||
-        ((reinterpret_cast<uintptr_t>(lse) | reinterpret_cast<uintptr_t>(delta)) & 3))
+    if (bad(dout) || bad(q) || bad(k) || bad(v) || bad(out) || bad(dq) || bad(dk) || bad(dv) || lse == nullptr || workspace == nullptr ||
+        (reinterpret_cast<uintptr_t>(lse) & 3) || (reinterpret_cast<uintptr_t>(workspace) & 15))
         return cudaErrorInvalidValue;
-    const unsigned grid_q = grid_for(p, TILE, p.heads), grid_k = grid_for(p, TILE, p.kv_heads);
-    const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads;
+    const int splits = splits_for(p);
+    const unsigned grid_q = grid_for(p, TILE, p.heads), grid_k = grid_for(p, TILE, p.kv_heads * splits);
+    const int64_t rows = static_cast<int64_t>(p.tokens) * p.heads, joined = 2 * static_cast<int64_t>(p.tokens) * p.kv_heads * (p.dim / 8);
+    float* delta = static_cast<float*>(workspace);
     CUtensorMap mq, mk, mv, mo;
-    if (grid_q == 0 || grid_k == 0 || (rows + 15) / 16 > 0x7fffffff || !make_map(&mq, q, p.heads, p) ||
+    if (grid_q == 0 || grid_k == 0 || (rows + 15) / 16 > 0x7fffffff || joined / 256 >= 0x7fffffff || !make_map(&mq, q, p.heads, p) ||
         !make_map(&mk, k, p.kv_heads, p) || !make_map(&mv, v, p.kv_heads, p) || !make_map(&mo, dout, p.heads, p))
         return cudaErrorInvalidValue;
     auto delta_go = [&](auto kernel) {
@@ -1342,6 +1432,8 @@ cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, T
     Params a = params(p);
     a.lse = const_cast<float*>(lse);
     a.delta = delta;
+    a.splits = splits;
+    a.part = delta + (rows + 3) / 4 * 4;
     return pick(p, [&](auto dp, auto half) {
         constexpr int DP = decltype(dp)::value;
         constexpr bool FP16 = decltype(half)::value;
@@ -1354,10 +1446,16 @@ cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, T
         const cudaError_t first = run<dkv_kernel<DP, FP16>>(grid_k, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
         if (first != cudaSuccess)
             return first;
-        a.out0 = static_cast<uint16_t*>(dq.p);
-        a.row0 = dq.row;
-        a.head0 = dq.head;
-        return run<dq_kernel<DP, FP16>>(grid_q, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, a);
+        Params b = a;
+        b.out0 = static_cast<uint16_t*>(dq.p);
+        b.row0 = dq.row;
+        b.head0 = dq.head;
+        const cudaError_t second = run<dq_kernel<DP, FP16>>(grid_q, BWD_THREADS, bwd_smem<DP>(), true, stream, mq, mk, mv, mo, b);
+        if (second != cudaSuccess || splits == 1)
+            return second;
+        join_kernel<FP16><<<static_cast<unsigned>((joined + 255) / 256), 256, 0, stream>>>(a);
+        count_launch();
+        return cudaGetLastError();
     });
 }
 

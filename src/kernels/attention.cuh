@@ -30,9 +30,10 @@ struct Problem {
 // out = softmax(scale q k^T) v, lse[head * tokens + row] = log of the sum of exponentials (natural)
 cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tensor out, float* lse, cudaStream_t stream);
 
-// `delta`: workspace of heads * tokens floats
+// `workspace`: backward_workspace(p) bytes, 16-byte aligned
+size_t backward_workspace(const Problem& p);
 cudaError_t launch_backward(const Problem& p, Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, const float* lse,
-                            Tensor dq, Tensor dk, Tensor dv, float* delta, cudaStream_t stream);
+                            Tensor dq, Tensor dk, Tensor dv, void* workspace, cudaStream_t stream);
 
 }  // namespace attn
 }  // namespace mgk

@@ -129,6 +129,13 @@ def test_long_sequences(causal, dtype, dim):
 
 
 @gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,heads,kv_heads", [([1900, 1800], 8, 8), ([1000, 30], 8, 1), ([1500], 6, 2), ([64] * 30, 4, 4)])
+def test_tiles_shared_and_not_shared_by_several_ctas(lengths, heads, kv_heads, causal):
+    run_and_check(lengths, heads, kv_heads, 64, BF, causal, tail=5, seed=11)
+
+
+@gpu
 @pytest.mark.parametrize("scale", [2.0 ** -20, 0.5, 3.0])
 def test_scales(scale):
     from megray_b200.ops import attention
@@ -350,5 +357,9 @@ def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
             assert fwd(a, *ts) == -1
     assert lib.megray_attention(a, t, t, t, t, None, None) == -1
     assert lib.megray_attention_bwd(a, t, t, t, t, t, None, t, t, t, 1024, None) == -1
+    assert lib.megray_attention_bwd(a, t, t, t, t, t, 1024, t, t, t, 1028, None) == -1
+    assert lib.megray_attention_bwd_workspace(a) >= 4 * 8
+    assert lib.megray_attention_bwd_workspace(_lib.AttnArgs(**{**ok, "dim": 60})) == 0
+    assert lib.megray_attention_bwd_workspace(_lib.AttnArgs(**{**ok, "tokens": 0})) == 0
     assert lib.megray_attention_bwd(a, t, t, t, t, t, 1024, t, t, t, None, None) == -1
     assert fwd(_lib.AttnArgs(**{**ok, "tokens": 0}), t, t, t, t) == 0
