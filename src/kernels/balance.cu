@@ -20,6 +20,7 @@
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
+#include "f32x2.cuh"
 #include "launch_count.h"
 
 namespace cg = cooperative_groups;
@@ -117,25 +118,95 @@ __host__ __device__ constexpr int rows_in_flight() {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// x <- x f + g;  sum of x y;  y <- y + x f: in pairs where there are pairs
+template <int NC, int VEC>
+__device__ __forceinline__ void scale_add(float (&x)[NC][VEC], float f, float g) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        if constexpr (VEC == 1) {
+            x[i][0] = fmaf(x[i][0], f, g);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VEC; v += 2) {
+                const f32x2::Pair p = f32x2::fma({x[i][v], x[i][v + 1]}, f32x2::both(f), f32x2::both(g));
+                x[i][v] = p.x;
+                x[i][v + 1] = p.y;
+            }
+        }
+    }
+}
+template <int NC, int VEC>
+__device__ __forceinline__ float dot_of(const float (&x)[NC][VEC], const float (&y)[NC][VEC]) {
+    if constexpr (VEC == 1) {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            d = fmaf(x[i][0], y[i][0], d);
+        return d;
+    } else {
+        f32x2::Pair d = f32x2::both(0.f);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; v += 2)
+                d = f32x2::fma({x[i][v], x[i][v + 1]}, {y[i][v], y[i][v + 1]}, d);
+        return d.x + d.y;
+    }
+}
+template <int NC, int VEC>
+__device__ __forceinline__ float sum_of(const float (&x)[NC][VEC]) {
+    if constexpr (VEC == 1) {
+        float d = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+            d += x[i][0];
+        return d;
+    } else {
+        f32x2::Pair d = f32x2::both(0.f);
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; v += 2)
+                d = f32x2::add(d, {x[i][v], x[i][v + 1]});
+        return d.x + d.y;
+    }
+}
+template <int NC, int VEC>
+__device__ __forceinline__ void add_scaled(float (&y)[NC][VEC], const float (&x)[NC][VEC], float f) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        if constexpr (VEC == 1) {
+            y[i][0] = fmaf(x[i][0], f, y[i][0]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VEC; v += 2) {
+                const f32x2::Pair p = f32x2::fma({x[i][v], x[i][v + 1]}, f32x2::both(f), {y[i][v], y[i][v + 1]});
+                y[i][v] = p.x;
+                y[i][v + 1] = p.y;
+            }
+        }
+    }
+}
+
 // x <- exp(x - top), with what is below the normal numbers as zero.  One fused step in front of 2^x; its rounding of
 // top log2e is the same in every term of a row and drops out where they are divided by their sum.  Where logits are
 // near the type's lowest number the product with log2e would overflow: there the difference comes first.
 template <int NC, int VEC>
 __device__ __forceinline__ void exponentials(float (&x)[NC][VEC], float top) {
-    const float t = top * LOG2E;
     if (fabsf(top) < 1e37f) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[i][v]) : "f"(fmaf(x[i][v], LOG2E, -t)));
+        scale_add<NC, VEC>(x, LOG2E, -top * LOG2E);
     } else {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
 #pragma unroll
             for (int v = 0; v < VEC; ++v)
-                asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[i][v]) : "f"((x[i][v] - top) * LOG2E));
+                x[i][v] = (x[i][v] - top) * LOG2E;
     }
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x[i][v]) : "f"(x[i][v]));
 }
 
 // Sums (or maxima) of U values over groups of W lanes, the U chains side by side
@@ -217,8 +288,11 @@ struct Walk {
         p = static_cast<const T*>(r.logits) + at * r.ld;
         mask = r.mask != nullptr ? r.mask + at : nullptr;
     }
-    __device__ __forceinline__ bool live(int u) const {
-        return u * per_warp < left && (mask == nullptr || mask[u * per_warp] != 0);
+    // which of the rows count
+    __device__ __forceinline__ void fetch(uint8_t (&live)[U]) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            live[u] = u * per_warp >= left ? 0 : mask == nullptr ? 1 : mask[u * per_warp];
     }
     __device__ __forceinline__ const T* row(int u) const { return p + u * u_step; }
     __device__ __forceinline__ void next() {
@@ -266,28 +340,52 @@ __device__ __forceinline__ void cta_stats(const Router& r, int W, int cta, int c
     // pairs, apart from the rows: contiguous whatever the number per token
     {
         const uint32_t pairs = static_cast<uint32_t>(r.tokens) * r.top, by = static_cast<uint32_t>(ctas) * kThreads;
-        for (uint32_t i = static_cast<uint32_t>(cta) * kThreads + threadIdx.x; i < pairs; i += by) {
-            const int64_t e = r.idx64 ? static_cast<const int64_t*>(r.idx)[i] : static_cast<const int*>(r.idx)[i];
-            if (e >= 0 && e < r.experts && (r.mask == nullptr || r.mask[i / static_cast<uint32_t>(r.top)] != 0))
-                atomicAdd(&s.counts[e], 1);
+        constexpr int AT_ONCE = 8;
+        for (uint64_t base = static_cast<uint64_t>(cta) * kThreads + threadIdx.x; base < pairs; base += static_cast<uint64_t>(by) * AT_ONCE) {
+            int64_t e[AT_ONCE];
+            uint8_t counts[AT_ONCE];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const uint64_t i = base + static_cast<uint64_t>(k) * by;
+                e[k] = -1;
+                counts[k] = 1;
+                if (i < pairs) {  // (the two loads do not wait for one another)
+                    e[k] = r.idx64 ? static_cast<const int64_t*>(r.idx)[i] : static_cast<const int*>(r.idx)[i];
+                    if (r.mask != nullptr)
+                        counts[k] = r.mask[static_cast<uint32_t>(i) / static_cast<uint32_t>(r.top)];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k)
+                if (counts[k] != 0 && e[k] >= 0 && e[k] < r.experts)
+                    atomicAdd(&s.counts[e[k]], 1);
         }
     }
     float acc[NC][VEC] = {};
     int valid = 0;
     Walk<T, VEC, NC> walk(r, W, cta, ctas);
     uint32_t raw[U][NC][words_of<T, VEC>()];
+    // rows that are on their way while others are worked on, and the masks of the rows after them: whether a row is read
+    // hangs on its mask
+    uint8_t live[U];
+    int next_at = 0, next_left = 0, next_of_warp = 0;
     auto load = [&]() {
+        next_at = walk.at;
+        next_left = walk.left;
+        next_of_warp = walk.left_of_warp;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool live = walk.live(u);
-            load_row<T, VEC, NC>(walk.row(u), live, W, sub, r.experts, raw[u]);
-            valid += live && sub == 0 ? 1 : 0;
+            load_row<T, VEC, NC>(walk.row(u), live[u] != 0, W, sub, r.experts, raw[u]);
+            valid += live[u] != 0 && sub == 0 ? 1 : 0;
         }
+        walk.next();
+        walk.fetch(live);
     };
+    walk.fetch(live);
     load();
     // (all lanes of a warp go round alike: the shuffles are warp-wide)
-    while (walk.left_of_warp > 0) {
-        const int at = walk.at, left = walk.left;
+    while (next_of_warp > 0) {
+        const int at = next_at, left = next_left;
         float x[U][NC][VEC], top[U], sum[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -296,28 +394,27 @@ __device__ __forceinline__ void cta_stats(const Router& r, int W, int cta, int c
 #pragma unroll
                 for (int v = 0; v < VEC; ++v)
                     x[u][i][v] = element<T, VEC>(raw[u][i], v);
-        walk.next();
-        load();  // the next rows, on their way while these are worked on
+        load();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             top[u] = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < NC; ++i)
+            for (int i = 0; i < NC; ++i) {
+                if constexpr (VEC == 1) {
+                    top[u] = fmaxf(top[u], x[u][i][0]);
+                } else {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    top[u] = fmaxf(top[u], x[u][i][v]);
+                    for (int v = 0; v < VEC; v += 2)
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(top[u]) : "f"(x[u][i][v]), "f"(x[u][i][v + 1]));
+                }
+            }
         }
         group_max<U>(top, W);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             top[u] = top[u] == -INFINITY ? 0.f : top[u];
             exponentials<NC, VEC>(x[u], top[u]);
-            sum[u] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    sum[u] += x[u][i][v];
+            sum[u] = sum_of<NC, VEC>(x[u]);
         }
         group_sum<U>(sum, W);
 #pragma unroll
@@ -325,11 +422,7 @@ __device__ __forceinline__ void cta_stats(const Router& r, int W, int cta, int c
             const float inv = sum[u] == 0.f ? 0.f : __fdividef(1.f, sum[u]);
             if (sub == 0 && u * per_warp < left)
                 rows[at + u * per_warp] = make_float2(top[u], inv);
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    acc[i][v] = fmaf(x[u][i][v], inv, acc[i][v]);
+            add_scaled<NC, VEC>(acc, x[u], inv);
         }
     }
     // groups of a warp that hold the same columns, then the warps of the CTA
@@ -421,22 +514,29 @@ __device__ __forceinline__ void cta_grads(const Router& r, const Result& out, in
     uint32_t raw[U][NC][words_of<T, VEC>()];
     float2 row[U];
     bool here[U];
+    uint8_t mask[U];
+    int next_at = 0, next_left = 0, next_of_warp = 0;
     auto load = [&]() {
+        next_at = walk.at;
+        next_left = walk.left;
+        next_of_warp = walk.left_of_warp;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            here[u] = walk.live(u);
-            row[u] = here[u] ? rows[walk.at + u * per_warp] : make_float2(0.f, 0.f);
+            here[u] = mask[u] != 0;
+            row[u] = u * per_warp < walk.left ? rows[walk.at + u * per_warp] : make_float2(0.f, 0.f);
             load_row<T, VEC, NC>(walk.row(u), here[u], W, sub, r.experts, raw[u]);
         }
+        walk.next();
+        walk.fetch(mask);
     };
+    walk.fetch(mask);
     load();
-    while (walk.left_of_warp > 0) {
-        const int at = walk.at, left = walk.left;
+    while (next_of_warp > 0) {
+        const int at = next_at, left = next_left;
         float x[U][NC][VEC], inv[U], dot[U];
         bool live[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            dot[u] = 0.f;
             live[u] = here[u];
             inv[u] = row[u].y;
 #pragma unroll
@@ -445,13 +545,8 @@ __device__ __forceinline__ void cta_grads(const Router& r, const Result& out, in
                 for (int v = 0; v < VEC; ++v)
                     x[u][i][v] = element<T, VEC>(raw[u][i], v);
             exponentials<NC, VEC>(x[u], row[u].x);
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    dot[u] = fmaf(x[u][i][v], w[i][v], dot[u]);
+            dot[u] = dot_of<NC, VEC>(x[u], w);
         }
-        walk.next();
         load();
         group_sum<U>(dot, W);
 #pragma unroll
@@ -465,10 +560,19 @@ __device__ __forceinline__ void cta_grads(const Router& r, const Result& out, in
                 const int c = (i * W + sub) * VEC;
                 if (c >= r.experts)
                     continue;
+                // p (w - dot) with p = x inv: x (w inv - dot inv)
                 float d[VEC];
+                if constexpr (VEC == 1) {
+                    d[0] = x[u][i][0] * fmaf(w[i][0], inv[u], -dot[u] * inv[u]);
+                } else {
 #pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    d[v] = x[u][i][v] * inv[u] * (w[i][v] - dot[u]);
+                    for (int v = 0; v < VEC; v += 2) {
+                        const f32x2::Pair q = f32x2::mul({x[u][i][v], x[u][i][v + 1]},
+                                                         f32x2::fma({w[i][v], w[i][v + 1]}, f32x2::both(inv[u]), f32x2::both(-dot[u] * inv[u])));
+                        d[v] = q.x;
+                        d[v + 1] = q.y;
+                    }
+                }
                 if (out.accumulate) {
                     float o[VEC];
                     load_old<VEC>(to + c, o);
@@ -482,9 +586,9 @@ __device__ __forceinline__ void cta_grads(const Router& r, const Result& out, in
     }
 }
 
-// (three CTAs on an SM where the registers of a row allow it)
+// (three CTAs on an SM, or two, where the registers of a row allow it)
 template <class T, int VEC, int NC>
-__global__ void __launch_bounds__(kThreads, VEC * NC <= 8 ? 3 : 1) __cluster_dims__(kCluster)
+__global__ void __launch_bounds__(kThreads, VEC * NC <= 16 ? 3 : VEC * NC <= 32 ? 2 : 1) __cluster_dims__(kCluster)
         stats_kernel(const Router r, int W, char* partial, float2* rows) {
     extern __shared__ __align__(16) char raw[];
     const Smem s = carve(raw, r.experts, true);
@@ -515,7 +619,7 @@ __global__ void __launch_bounds__(kThreads, VEC * NC <= 8 ? 3 : 1) __cluster_dim
 }
 
 template <class T, class D, int VEC, int NC>
-__global__ void __launch_bounds__(kThreads, VEC * NC <= 8 ? 3 : 1) __cluster_dims__(kCluster)
+__global__ void __launch_bounds__(kThreads, VEC * NC <= 16 ? 3 : VEC * NC <= 32 ? 2 : 1) __cluster_dims__(kCluster)
         grad_kernel(const Router r, int W, const char* partial, int n_partials, const float2* rows, const Result out) {
     extern __shared__ __align__(16) char raw[];
     const Smem s = carve(raw, r.experts, false);
@@ -599,11 +703,14 @@ Shape shape(const Router& r, const Result* out) {
     Shape s;
     s.vec = r.bf16 && vectors(r, out, 8) ? 8 : vectors(r, out, 4) ? 4 : 1;
     const int units = (r.experts + s.vec - 1) / s.vec;
+    // Two vectors a lane before more lanes: a warp then has more rows, and what is done once a row, the sums over lanes
+    // above all, is done for all of them at once.  (More take the registers of other warps: 200003 x 256 bf16 logits
+    // 105 us with one vector, 136 with four.)
     s.W = 1;
-    while (s.W < 32 && s.W < units)
+    while (s.W < 32 && s.W * 2 < units)
         s.W *= 2;
     s.nc = 1;
-    while (s.nc * 32 < units)
+    while (s.nc * s.W < units)
         s.nc *= 2;
     return s;
 }
