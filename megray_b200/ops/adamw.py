@@ -39,6 +39,9 @@ class AdamWState:
             raise ValueError("AdamWState: moments are kept in 8 or in 32 bits")
         if not params or any(not p.is_cuda or p.device != params[0].device for p in params):
             raise ValueError("AdamWState: expected CUDA tensors of one device")
+        places = [p.data_ptr() for p in params if p.numel()]
+        if len(set(places)) < len(places):
+            raise ValueError("AdamWState: a tensor is in the list twice")
         self.bits, self.device = bits, params[0].device
         self.sizes = [p.numel() for p in params]
         blocks = np.array([-(-n // BLOCK) for n in self.sizes], dtype=np.uint64)

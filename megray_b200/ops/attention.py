@@ -4,7 +4,8 @@ Prompts lie one behind the other in the rows of ``[T, heads, D]`` tensors; ``cu_
 ``[0, L0, L0 + L1, ...]``) says where each begins.  A query sees the keys of its own prompt, with ``causal`` those up to
 its own position.  Key / value heads may be fewer than query heads: query head h reads key / value head
 ``h * Hk // H``.  bf16 or float16, D a multiple of 8 up to 128, any strides that are multiples of 8 elements
-(slices of one projection among them).
+(slices of one projection among them).  A wait inside a kernel that runs out sets the word of
+:func:`megray_b200.ops.gemm_error_flag`.
 """
 from __future__ import annotations
 
@@ -59,6 +60,8 @@ def _problem(q, k, v, cu_seqlens, causal, scale):
     kv_heads, dtype, index = k.shape[1], q.dtype, q.get_device()
     if dim & 7 or not 8 <= dim <= 128 or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("attention: D is a multiple of 8 from 8 to 128, the query heads a multiple of the key heads")
+    if tokens >= 2 ** 31:
+        raise ValueError("attention: fewer than 2^31 rows")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     elif not 0.0 < scale < math.inf:
@@ -101,6 +104,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     args, cq, ck, cv, index = _problem(q, k, v, cu_seqlens, causal, scale)
     partly = cu_seqlens is not None
     out, co = _output(out, args.tokens, args.heads, args.dim, q, index, partly, "out")
+    if co.p is not None and co.p in (ck.p, cv.p):
+        raise ValueError("attention: out lies where the keys or values do")
     if lse is None and partly:
         lse = q.new_zeros(args.heads, args.tokens, dtype=torch.float32)
     lse = _row_sums(lse, args.heads, args.tokens, q, index, "lse")
@@ -116,7 +121,8 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     """Returns (dq, dk, dv) for the gradient ``dout`` of the ``out`` that :func:`attention` returned with ``lse`` for the
     same arguments.  Gradients of key / value heads are summed over the query heads that read them.  Given tensors
     are written to (any of the strides that the inputs may have, slices of one buffer among them); rows behind the
-    last prompt are left as they are (zeros in tensors made here).  No atomics: the same inputs give the same bits."""
+    last prompt are left as they are (zeros in tensors made here).  They may not overlap the inputs, which are read until
+    the end.  No atomics: the same inputs give the same bits."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention_bwd(dout, q, k, v, out, lse, cu_seqlens, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)
@@ -130,6 +136,8 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     dq, cdq = _output(dq, tokens, heads, dim, q, index, cu_seqlens is not None, "dq")
     dk, cdk = _output(dk, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dk")
     dv, cdv = _output(dv, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dv")
+    if tokens and not {cdq.p, cdk.p, cdv.p}.isdisjoint((cd.p, cq.p, ck.p, cv.p, co.p)):
+        raise ValueError("attention_bwd: a gradient lies where an input does")
     lib = _lib.load()
     room = q.new_empty(lib.megray_attention_bwd_workspace(args), dtype=torch.uint8)
     rc = lib.megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, room.data_ptr(), raw_stream(index))

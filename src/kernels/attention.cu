@@ -219,41 +219,35 @@ struct Where {
     int start, len, local;  // first row and length of the sequence, the tile's number in it; len = 0: no such tile
     int tiles;              // tiles of the sequence
 };
-// By one whole warp.  Offsets are forced into order and range, so that no access leaves the tensors
-// whatever they hold.
+// Tiles are numbered so that a sequence's first one follows from its own offset alone: tile cu[s] / rows + s.  (A sequence
+// of L rows takes at most L / rows + 1 numbers, and the next one begins no earlier.)  So the sequence of a tile is found
+// by a search, 32 offsets a step, whatever the number of sequences; numbers in between belong to no tile.  By one
+// whole warp.  Offsets are forced into order and range, so that no access leaves the tensors whatever they hold.
 __device__ __forceinline__ Where find_tile(const Params& p, int rows, int index) {
     Where w{0, 0, 0, 0};
-    const int lane = threadIdx.x & 31;
     if (p.cu == nullptr) {
         w.tiles = (p.tokens + rows - 1) / rows;
         if (index < w.tiles)
             w = {0, p.tokens, index, w.tiles};
         return w;
     }
-    for (int base = 0; base < p.seqs; base += 32) {
-        const int s = base + lane;
-        int a = 0, e = 0;
-        if (s < p.seqs) {
-            a = min(max(p.cu[s], 0), p.tokens);
-            e = min(max(p.cu[s + 1], a), p.tokens);
-        }
-        const int n = (e - a + rows - 1) / rows;
-        int upto = n;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o)
-                upto += v;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, upto > index);
-        if (past != 0) {
-            const int src = __ffs(past) - 1;
-            w.start = __shfl_sync(0xffffffffu, a, src);
-            w.len = __shfl_sync(0xffffffffu, e, src) - w.start;
-            w.tiles = __shfl_sync(0xffffffffu, n, src);
-            w.local = index - (__shfl_sync(0xffffffffu, upto, src) - w.tiles);
+    const int lane = threadIdx.x & 31;
+    auto offset = [&](int s) { return min(max(p.cu[s], 0), p.tokens); };
+    int lo = 0, hi = p.seqs;  // the last sequence that begins at or before the tile lies in [lo, hi)
+    do {
+        const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+        const unsigned before = __ballot_sync(0xffffffffu, s < hi && offset(s) / rows + s <= index);
+        if (before == 0)
             return w;
-        }
-        index -= __shfl_sync(0xffffffffu, upto, 31);
+        lo += (31 - __clz(before)) * step;
+        hi = min(hi, lo + step);
+    } while (hi - lo > 1);
+    const int start = offset(lo), len = max(offset(lo + 1) - start, 0);
+    w.tiles = (len + rows - 1) / rows;
+    w.local = index - (start / rows + lo);
+    if (w.local >= 0 && w.local < w.tiles) {
+        w.start = start;
+        w.len = len;
     }
     return w;
 }
@@ -559,7 +553,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             Pair sum[2];
             // P with the maximum as it is, the block's own maximum beside it; a chunk is loaded while one is worked on
             auto exponentials = [&]() {
-                const Pair cc = both(c), mc = both(-m * c);
+                // (where all scores so far were -infinity their exponentials are zero)
+                const Pair cc = both(c), mc = both(m == -INFINITY ? 0.f : -m * c);
                 float top[2] = {-INFINITY, -INFINITY};
                 sum[0] = sum[1] = both(0.f);
                 tmem_ld_32x32b_x32(s_at, s[0]);
@@ -595,7 +590,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             } else {
                 const float mx = exponentials();
                 // each row goes by its own maximum (also where a score is NaN: the row becomes NaN)
-                const bool rises = !((mx - m) * c <= (FP16 ? 8.f : 32.f)) && row < w.len;
+                const bool rises = !((mx - m) * c <= (FP16 ? 8.f : 32.f)) && mx != -INFINITY && row < w.len;
                 if (__any_sync(0xffffffffu, rises)) {
                     // the product that last added to O has retired: the scores' barrier came after it
                     const float to = rises ? max3_nan(m, mx, mx) : m, f = ex2((m - to) * c);
@@ -1283,13 +1278,10 @@ bool bad(const Problem& p) {
            p.seqs < 0 || (p.cu != nullptr && p.seqs < 1) || (reinterpret_cast<uintptr_t>(p.cu) & 3) || !(p.scale > 0.f) ||
            !(p.scale < INFINITY);
 }
-// CTAs that cover every possible cut of the rows into sequences, `rows` of one sequence and `heads` heads each;
-// 0 when there are too many
+// CTAs for the tiles of `rows` rows that find_tile numbers, `heads` for each; 0 when there are too many
 unsigned grid_for(const Problem& p, int rows, int heads) {
-    const int64_t seqs = p.cu != nullptr ? p.seqs : 1;
-    const int64_t tiles = (p.tokens + seqs * (rows - 1)) / rows;
-    const int64_t most = p.tokens < tiles ? p.tokens : tiles;
-    const int64_t ctas = (p.cu != nullptr ? most : (p.tokens + rows - 1) / rows) * heads;
+    const int64_t tiles = p.cu != nullptr ? static_cast<int64_t>(p.tokens) / rows + p.seqs : (p.tokens + rows - 1) / rows;
+    const int64_t ctas = tiles * heads;
     return ctas > 0x7fffffff ? 0u : static_cast<unsigned>(ctas);
 }
 Params params(const Problem& p) {

@@ -760,6 +760,8 @@ float2* rows_of(void* workspace, const Router& r) {
 }  // namespace
 
 size_t workspace_bytes(int tokens, int experts) {
+    if (tokens < 0 || experts < 1)
+        return 0;
     return static_cast<size_t>(kMaxPartials) * partial_words(experts) * 4 + static_cast<size_t>(tokens) * sizeof(float2);
 }
 

@@ -196,6 +196,8 @@ def test_refusals():
             adamw_step(kw.pop("params"), kw.pop("grads"), state, kw.pop("lr"), **kw)
     with pytest.raises(ValueError):
         AdamWState(params, bits=16)
+    with pytest.raises(ValueError):
+        AdamWState([params[0], params[0]])
     state.m = state.m[:-1]
     with pytest.raises(ValueError):
         adamw_step(params, grads, state, step=1, **H)

@@ -191,6 +191,47 @@ def test_strided_operands():
 
 
 @gpu
+@pytest.mark.parametrize("count", [31, 32, 33, 200, 1023, 1500])
+def test_more_sequences_than_a_search_step_holds(count):
+    g = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 4, (count,), generator=g).tolist()
+    lengths[count // 2] = 300
+    run_and_check(lengths, 2, 1, 16, BF, True, tail=7)
+
+
+@gpu
+def test_rows_that_are_no_multiple_of_the_heads():
+    from megray_b200.ops import attention, attention_bwd
+
+    rows, h, d = 150, 4, 32
+    store = torch.randn(rows, h * d + 8, device="cuda").to(BF)
+    x = store[:, :h * d].view(rows, h, d)
+    out, lse = attention(x, x, x)
+    plain = x.contiguous()
+    want, want_lse = attention(plain, plain, plain)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    for a, b in zip(attention_bwd(out, x, x, x, out, lse), attention_bwd(want, plain, plain, plain, want, want_lse)):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("hidden", [100, 128, 200, 300])
+def test_scores_of_minus_infinity(hidden):
+    """Keys that give a score of -infinity to every query have no weight, also where they fill the first blocks."""
+    from megray_b200.ops import attention
+
+    n = 400
+    q, k, v, _ = make([n], 1, 1, 64, BF, seed=2)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[:hidden, :, 0] = float("-inf")
+    out, lse = attention(q, k, v, causal=False)
+    z = q[:, 0].double() @ k[hidden:, 0].double().t() / 8
+    p = torch.softmax(z, 1)
+    check(out[:, 0], p @ v[hidden:, 0].double(), p @ v[hidden:, 0].double().abs(), BF, "out")
+    assert bool(((lse[0].double() - torch.logsumexp(z, 1)).abs() <= 2.0 ** -14).all())
+
+
+@gpu
 def test_other_sequences_do_not_matter():
     from megray_b200.ops import attention, attention_bwd
 
@@ -320,7 +361,11 @@ def test_refusals():
     with pytest.raises(ValueError):
         attention(big, big, big)
     out, lse = attention(q, k, v, cu)
-    for bad in (dict(dout=do[:5]), dict(dout=do.half()), dict(out=None), dict(lse=None), dict(lse=lse[:2]), dict(dk=q), dict(dq=k)):
+    for same in (k, v):
+        with pytest.raises(ValueError):
+            attention(k, k, v, cu, out=same)
+    for bad in (dict(dout=do[:5]), dict(dout=do.half()), dict(out=None), dict(lse=None), dict(lse=lse[:2]), dict(dk=q), dict(dq=k),
+                dict(dq=q), dict(dq=do), dict(dk=v)):
         kw = {"dout": do, "out": out, "lse": lse, **bad}
         with pytest.raises(ValueError):
             attention_bwd(kw.pop("dout"), q, k, v, kw.pop("out"), kw.pop("lse"), cu, **kw)
