@@ -197,6 +197,7 @@ typedef struct {
     float scale;
     int* error_flag;      /* device word, set to 1 when a wait inside a kernel runs out; or null */
 } megray_attn_args;
+/* What is written overlaps neither an input nor another result; only out may be q itself, strides and all. */
 int megray_attention(const megray_attn_args* a, const megray_attn_tensor* q, const megray_attn_tensor* k,
                      const megray_attn_tensor* v, const megray_attn_tensor* out, float* lse, void* stream);
 int megray_attention_bwd(const megray_attn_args* a, const megray_attn_tensor* dout, const megray_attn_tensor* q,

@@ -97,15 +97,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     rise from 0 to at most T; nothing outside the tensors is touched if it does not, but rows may then go
     unwritten.  Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32.  A NaN or
     an infinity in the values of a prompt may reach any row of that prompt, those of other prompts and of rows
-    behind the last never do."""
+    behind the last never do.  ``out`` may be ``q`` itself (the queries are then gone, also for the backward pass); beside
+    that neither result may overlap an input or the other."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention(q, k, v, cu_seqlens, causal=causal, scale=scale, out=out, lse=lse)
     args, cq, ck, cv, index = _problem(q, k, v, cu_seqlens, causal, scale)
     partly = cu_seqlens is not None
     out, co = _output(out, args.tokens, args.heads, args.dim, q, index, partly, "out")
-    if co.p is not None and co.p in (ck.p, cv.p):
-        raise ValueError("attention: out lies where the keys or values do")
+    if co.p is not None and (co.p in (ck.p, cv.p) or co.p == cq.p and (co.row, co.head) != (cq.row, cq.head)):
+        raise ValueError("attention: out lies where the keys or values do, or on the queries in another order")
     if lse is None and partly:
         lse = q.new_zeros(args.heads, args.tokens, dtype=torch.float32)
     lse = _row_sums(lse, args.heads, args.tokens, q, index, "lse")
@@ -121,8 +122,8 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     """Returns (dq, dk, dv) for the gradient ``dout`` of the ``out`` that :func:`attention` returned with ``lse`` for the
     same arguments.  Gradients of key / value heads are summed over the query heads that read them.  Given tensors
     are written to (any of the strides that the inputs may have, slices of one buffer among them); rows behind the
-    last prompt are left as they are (zeros in tensors made here).  They may not overlap the inputs, which are read until
-    the end.  No atomics: the same inputs give the same bits."""
+    last prompt are left as they are (zeros in tensors made here).  They may overlap neither the inputs, which are read
+    until the end, nor one another.  No atomics: the same inputs give the same bits."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention_bwd(dout, q, k, v, out, lse, cu_seqlens, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)
@@ -138,6 +139,8 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     dv, cdv = _output(dv, tokens, kv_heads, dim, q, index, cu_seqlens is not None, "dv")
     if tokens and not {cdq.p, cdk.p, cdv.p}.isdisjoint((cd.p, cq.p, ck.p, cv.p, co.p)):
         raise ValueError("attention_bwd: a gradient lies where an input does")
+    if tokens and len({cdq.p, cdk.p, cdv.p}) < 3:
+        raise ValueError("attention_bwd: two gradients lie in one place")
     lib = _lib.load()
     room = q.new_empty(lib.megray_attention_bwd_workspace(args), dtype=torch.uint8)
     rc = lib.megray_attention_bwd(args, cd, cq, ck, cv, co, lse.data_ptr(), cdq, cdk, cdv, room.data_ptr(), raw_stream(index))

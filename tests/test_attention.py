@@ -371,6 +371,35 @@ def test_refusals():
             attention_bwd(kw.pop("dout"), q, k, v, kw.pop("out"), kw.pop("lse"), cu, **kw)
 
 
+@gpu
+def test_results_in_one_place_are_refused():
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([64], 2, 2, 64, BF)
+    out, lse = attention(q, k, v)
+    both, third = torch.empty_like(k), torch.empty_like(k)
+    for grads in (dict(dk=both, dv=both), dict(dq=both, dk=both), dict(dq=both, dk=third, dv=both)):
+        with pytest.raises(ValueError):
+            attention_bwd(do, q, k, v, out, lse, **grads)
+    attention_bwd(do, q, k, v, out, lse, dq=torch.empty_like(q), dk=both, dv=third)
+    other = q.as_strided(q.shape, (64, 64 * 64, 1))  # the same memory, head by head
+    with pytest.raises(ValueError):
+        attention(q, k, v, out=other)
+
+
+@gpu
+@pytest.mark.parametrize("lens,heads,kv_heads,causal", [([1], 2, 2, True), ([200, 1, 129, 70], 4, 2, False), ([2500, 40, 1300], 16, 4, True)])
+def test_the_output_may_take_the_place_of_the_queries(lens, heads, kv_heads, causal):
+    from megray_b200.ops import attention
+
+    q, k, v, _ = make(lens, heads, kv_heads, 64, BF)
+    cu = ends(lens)
+    want, want_lse = attention(q, k, v, cu, causal=causal)
+    over = q.clone()
+    got, lse = attention(over, k, v, cu, causal=causal, out=over)
+    assert got is over and torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
 def test_cpu_tensors_are_refused():
     from megray_b200.ops import attention, attention_bwd
 
