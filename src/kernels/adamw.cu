@@ -173,9 +173,10 @@ __device__ __forceinline__ float rcp_approx(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// Square roots of eight numbers, exact but for a few in a million that are one float32 step off: the approximate
-// reciprocal root and one correction by the exact residual.  Zeros, numbers near the denormal ones and infinities
-// take CUDA's function.
+// Square roots of eight numbers by one step of Newton's method for s^2 = x, that is s + (x - s^2) / (2 s), from
+// s = x y with the hardware's approximate y = 1 / sqrt(x): a relative error e of s becomes e^2 / 2, so what is left is the
+// last rounding, at most one float32 step.  Zeros, numbers near the denormal ones and infinities take CUDA's
+// function.
 __device__ __forceinline__ void roots8(const float (&v)[8], float (&r)[8]) {
     const float lo = fminf(min3(v[0], v[1], v[2]), fminf(min3(v[3], v[4], v[5]), fminf(v[6], v[7])));
     const float hi = fmaxf(max3(v[0], v[1], v[2]), fmaxf(max3(v[3], v[4], v[5]), fmaxf(v[6], v[7])));

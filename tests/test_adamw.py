@@ -132,6 +132,24 @@ def test_zero_missing_and_bad_gradients(bits):
 
 
 @gpu
+@pytest.mark.parametrize("reach", [40, 60])  # 60 goes past the range of the root's own iteration
+def test_roots_against_float64(reach):
+    """A block's scale of r is its largest root over 448: the root is at most one float32 step off (2 U of its value),
+    1 / 448 and the product half a step each."""
+    from megray_b200.ops import AdamWState, adamw_step
+
+    g = torch.Generator(device="cuda").manual_seed(3)
+    blocks = 20_000
+    x = (1 + torch.rand(blocks, device="cuda", generator=g)) * 2.0 ** torch.randint(-reach, reach, (blocks,), device="cuda", generator=g)
+    grad, param = x[:, None].expand(blocks, 256).reshape(-1).contiguous(), torch.zeros(blocks * 256, device="cuda")
+    state = AdamWState([param], bits=8)
+    adamw_step([param], [grad], state, 1e-3, step=1, betas=(0.9, 0.95))
+    v = (x * x) * torch.tensor(1.0 - 0.95, dtype=torch.float32, device="cuda")
+    want = v.double().sqrt() / 448
+    assert ((state.r_scale.double() - want).abs() <= 4 * U * (1 + 1e-6) * want).all()
+
+
+@gpu
 def test_mixed_types_and_nothing_to_do():
     from megray_b200.ops import AdamWState, adamw_step
 
