@@ -189,11 +189,12 @@ __device__ __forceinline__ void add_scaled(float (&y)[NC][VEC], const float (&x)
 }
 
 // x <- exp(x - top), with what is below the normal numbers as zero.  One fused step in front of 2^x; its rounding of
-// top log2e is the same in every term of a row and drops out where they are divided by their sum.  Where logits are
-// near the type's lowest number the product with log2e would overflow: there the difference comes first.
+// top log2e is the same in every term of a row and drops out where they are divided by their sum, as long as 2 to the
+// power of that error is an ordinary number: at |top| < 2^20 the error is below 2^-3.  (From 1.5e9 on it would pass 128.)
+// Beyond, the difference comes first: it is exact for what is near top, and for the rest too large to count.
 template <int NC, int VEC>
 __device__ __forceinline__ void exponentials(float (&x)[NC][VEC], float top) {
-    if (fabsf(top) < 1e37f) {
+    if (fabsf(top) < 0x1p20f) {
         scale_add<NC, VEC>(x, LOG2E, -top * LOG2E);
     } else {
 #pragma unroll

@@ -237,3 +237,23 @@ def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
     assert lib.megray_balance(r, out, None, None) == -1 and lib.megray_balance(r, out, 72, None) == -1
     for bad in ((None, 64, 64, 8, 7), (64, None, 64, 8, 7), (64, 64, 66, 8, 7), (64, 64, 64, 7, 7), (64, 64, 64, 8, 10)):
         assert lib.megray_balance(r, _lib.BalanceOut(*bad, 0, 1.0), 64, None) == -1, bad
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,experts", [(300, 8), (700, 33), (40_000, 12), (3000, 256)])
+@pytest.mark.parametrize("size", [1e6, 1e9, 1e10, 1e12, 1e30])
+def test_rows_of_large_logits(size, tokens, experts, dtype):
+    """Softmax does not change with a constant added to a row: rows at +-size are as evenly spread as rows at zero, and
+    single entries there take all of a row or none of it."""
+    from megray_b200.ops import balance_loss_grad
+
+    logits, idx = make(tokens, experts, 2, dtype)
+    last = experts - 1
+    logits[3], logits[4] = size, -size
+    logits[5, last], logits[6, 1] = size, -size
+    logits[7], logits[8] = -size, size
+    logits[7, 2], logits[8, 2] = size, -size
+    logits[9, :2], logits[9, 2:] = size, -size          # two that share a row
+    logits[tokens - 1] = -size
+    close(balance_loss_grad(logits, idx, 0.01), reference(logits, idx, 0.01))
