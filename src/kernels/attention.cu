@@ -940,8 +940,13 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     constexpr int TB = tile_bytes<DP>();
     // K, V, then Q slots, then dO slots, then -lse log2 e and -delta of the rows of two blocks
     extern __shared__ __align__(1024) uint8_t smem[];
-    if (unaligned(smem, p))
+    // dQ's last CTA waits for this kernel alone, and what comes after dQ relies on delta's end too: also where no CTA
+    // has a tile (empty sequences only), the last one waits for delta.
+    const bool ends_last = blockIdx.x == gridDim.x - 1;
+    if (unaligned(smem, p)) {
+        wait_for_last_kernel();
         return;
+    }
     uint8_t *ring_q = smem + 2 * TB, *ring_do = ring_q + LONG_STAGES * TB;
     float* stats = reinterpret_cast<float*>(ring_do + SHORT_STAGES * TB);
     uint64_t* bars = reinterpret_cast<uint64_t*>(stats + SHORT_STAGES * 2 * TILE);
@@ -1002,6 +1007,8 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     if (w.len == 0) {  // no such tile
         if (warp == MMA_WARP)
             tmem_dealloc_cg1(tmem, 512);
+        if (ends_last)
+            wait_for_last_kernel();
         return;
     }
     const uint32_t t_a = tmem, t_p = tmem + TILE, t_ds = t_p + 64, t_dv = tmem + 2 * TILE, t_dk = tmem + 3 * TILE;

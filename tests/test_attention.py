@@ -437,3 +437,20 @@ def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
     assert lib.megray_attention_bwd_workspace(_lib.AttnArgs(**{**ok, "tokens": 0})) == 0
     assert lib.megray_attention_bwd(a, t, t, t, t, t, 1024, t, t, t, None, None) == -1
     assert fwd(_lib.AttnArgs(**{**ok, "tokens": 0}), t, t, t, t) == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows,heads,kv_heads", [(60_000, 32, 8), (2000, 8, 1)])
+def test_nothing_is_under_way_after_a_backward_pass_over_empty_sequences(rows, heads, kv_heads):
+    """The workspace goes back to the allocator with the call: what is put in its place on the same stream stays."""
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([], heads, kv_heads, 64, BF, tail=rows)
+    cu = torch.zeros(5, dtype=torch.int32, device="cuda")
+    out, lse = attention(q, k, v, cu)
+    for _ in range(10):
+        grads = attention_bwd(do, q, k, v, out, lse, cu)
+        next_ones = [torch.full((heads, rows), 7.0, device="cuda") for _ in range(3)]
+        assert all(bool((t == 7.0).all()) for t in next_ones)
+        assert all(not bool(g.any()) for g in grads)
+    assert not bool(out.any()) and not bool(lse.any())
