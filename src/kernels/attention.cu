@@ -601,7 +601,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                 const bool rises = !((mx - m) * c <= (FP16 ? 8.f : 32.f)) && mx != -INFINITY && row < w.len;
                 if (__any_sync(0xffffffffu, rises)) {
                     // the product that last added to O has retired: the scores' barrier came after it
-                    const float to = rises ? max3_nan(m, mx, mx) : m, f = ex2((m - to) * c);
+                    // (a row that does not rise is left alone: its maximum may be -infinity still)
+                    const float to = rises ? max3_nan(m, mx, mx) : m, f = rises ? ex2((m - to) * c) : 1.f;
                     m = to;
                     l *= f;
                     for (int d = 0; d < p.dim; d += 32) {

@@ -454,3 +454,41 @@ def test_nothing_is_under_way_after_a_backward_pass_over_empty_sequences(rows, h
         assert all(bool((t == 7.0).all()) for t in next_ones)
         assert all(not bool(g.any()) for g in grads)
     assert not bool(out.any()) and not bool(lse.any())
+
+
+@gpu
+def test_rows_whose_scores_are_minus_infinity_beside_others():
+    """Causal queries in front of the first key that has a weight: nothing to divide by, and the rows behind them, in
+    the same warps, are as without the keys in front."""
+    from megray_b200.ops import attention
+
+    n, hidden = 400, 130
+    q, k, v, _ = make([n], 1, 1, 64, BF, seed=2)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[:hidden, :, 0] = float("-inf")
+    out, lse = attention(q, k, v, causal=True)
+    assert bool(torch.isneginf(lse[0, :hidden]).all()) and bool(torch.isnan(out[:hidden]).all())
+    z = q[hidden:, 0].double() @ k[hidden:, 0].double().t() / 8
+    z = z.masked_fill(torch.ones_like(z, dtype=torch.bool).triu(1), -math.inf)
+    p = torch.softmax(z, 1)
+    check(out[hidden:, 0], p @ v[hidden:, 0].double(), p @ v[hidden:, 0].double().abs(), BF, "out")
+    assert bool(((lse[0, hidden:].double() - torch.logsumexp(z, 1)).abs() <= 2.0 ** -14).all())
+
+
+@gpu
+def test_scores_that_overflow_for_every_other_query():
+    """The first 256 keys score -infinity for even queries; for odd ones the second block outweighs the first by far, so
+    that half the rows of every warp rescale what the others have not begun."""
+    from megray_b200.ops import attention
+
+    n = 512
+    q, k, v, _ = make([n], 1, 1, 64, BF, seed=4)
+    q[..., :2] = k[..., :2] = 0.0
+    q[::2, :, 0], k[:256, :, 0] = 2.0 ** 100, -2.0 ** 100
+    q[1::2, :, 1], k[128:256, :, 1] = 8.0, 200.0
+    out, lse = attention(q, k, v, causal=False)
+    z = q[:, 0].double() @ k[:, 0].double().t() / 8
+    z[::2, :256] = -math.inf
+    p = torch.softmax(z, 1)
+    check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs(), BF, "out")
+    assert bool(((lse[0].double() - torch.logsumexp(z, 1)).abs() <= 2.0 ** -12).all())  # scores up to 200
