@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "f32x2.cuh"
 #include "gemm_device.cuh"
@@ -42,6 +43,7 @@ constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 elements
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int POLY = 1, POLY_OF = 4;  // of so many pairs of exponentials, so many by polynomial
 constexpr uint64_t WAIT_NS = 4000000000ull;
+constexpr float FAR = 0x1p20f;  // scores times scale log2 e from which on exponents are formed from differences
 
 struct Params {
     const int* cu;
@@ -560,9 +562,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
             uint32_t s[2][32], pk[2][32];
             Pair sum[2];
             // P with the maximum as it is, the block's own maximum beside it; a chunk is loaded while one is worked on
-            auto exponentials = [&]() {
+            auto exponentials = [&](auto far) {
+                constexpr bool FAR_ROWS = decltype(far)::value;
                 // (where all scores so far were -infinity their exponentials are zero)
-                const Pair cc = both(c), mc = both(m == -INFINITY ? 0.f : -m * c);
+                const float base = m == -INFINITY ? 0.f : m;
+                // a row is far or not by itself, so that all its blocks have one reference
+                const bool apart = FAR_ROWS && fabsf(base * c) >= FAR;
+                const Pair cc = both(c), mc = both(apart ? 0.f : -base * c), off = both(apart ? -base : 0.f);
                 float top[2] = {-INFINITY, -INFINITY};
                 sum[0] = sum[1] = both(0.f);
                 tmem_ld_32x32b_x32(s_at, s[0]);
@@ -574,7 +580,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float a = __uint_as_float(s[i & 1][2 * e]), b = __uint_as_float(s[i & 1][2 * e + 1]);
-                        Pair x = f32x2::fma({a, b}, cc, mc);
+                        Pair x = f32x2::fma(FAR_ROWS ? f32x2::add({a, b}, off) : Pair{a, b}, cc, mc);
                         x = e % POLY_OF < POLY ? ex2_pair<true>(x) : ex2_pair<false>(x);
                         top[e & 1] = max3_nan(top[e & 1], a, b);
                         sum[e & 1] = f32x2::add(sum[e & 1], x);
@@ -594,9 +600,9 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                         top = max3_nan(top, __uint_as_float(s[0][e]), __uint_as_float(s[0][e + 1]));
                 }
                 m = top;
-                exponentials();
+                exponentials(std::false_type{});
             } else {
-                const float mx = exponentials();
+                const float mx = exponentials(std::false_type{});
                 // each row goes by its own maximum (also where a score is NaN: the row becomes NaN)
                 const bool rises = !((mx - m) * c <= (FP16 ? 8.f : 32.f)) && mx != -INFINITY && row < w.len;
                 if (__any_sync(0xffffffffu, rises)) {
@@ -613,9 +619,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 1)
                             s[0][e] = __float_as_uint(__uint_as_float(s[0][e]) * f);
                         tmem_st_x32(o_at + d, s[0]);
                     }
-                    exponentials();
+                    exponentials(std::false_type{});
                 }
             }
+            // Far from zero the rounding of m c alone is a whole exponent: there the difference comes first
+            if (__any_sync(0xffffffffu, fabsf(m * c) >= FAR && fabsf(m) != INFINITY && row < w.len))
+                exponentials(std::true_type{});
             tmem_st_x32(s_at, pk[0]);
             tmem_st_x32(s_at + 32, pk[1]);
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);

@@ -492,3 +492,27 @@ def test_scores_that_overflow_for_every_other_query():
     p = torch.softmax(z, 1)
     check(out[:, 0], p @ v[:, 0].double(), p @ v[:, 0].double().abs(), BF, "out")
     assert bool(((lse[0].double() - torch.logsumexp(z, 1)).abs() <= 2.0 ** -12).all())  # scores up to 200
+
+
+@gpu
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype,size,scale", [(BF, 2.0 ** 11, None), (BF, 2.0 ** 17, None), (BF, 2.0 ** 40, 0.3), (BF, 2.0 ** 62, None),
+                                              (HF, 2.0 ** 14, 2.0 ** 8)])
+@pytest.mark.parametrize("first", [100, 128, 300])
+def test_finite_scores_of_any_size(first, dtype, size, scale, causal, sign):
+    """Scores far from zero, exact in float32: keys with the same one share a row evenly, those far below have no part in it,
+    whichever come first."""
+    from megray_b200.ops import attention
+
+    n = 500
+    q, k, v, _ = make([n], 2, 1, 64, dtype, seed=6)
+    q[::2], q[1::2, :, 0] = 0.0, 0.0  # odd queries see ordinary scores
+    q[::2, :, 0], k[:, :, 0] = size * 1.0078125, 0.0
+    k[:first, :, 0] = sign * size * 1.3359375
+    out, lse = attention(q, k, v, causal=causal, scale=scale)
+    val, weight, want = reference(q, k, v, q, [n], causal, scale)
+    off = 64 * 16.0 * (0 if scale is None else scale) * 2.0 ** -22  # ordinary scores times a large scale
+    tol = val["out"].abs() * HALF[dtype] + weight["out"] * (HALF[dtype] + 2 * off + 2.0 ** -13) * 1.01 + (2.0 ** -24 if dtype == HF else 0.0)
+    assert bool(((out.double() - val["out"]).abs() <= tol).all())
+    assert bool(((lse.double() - want).abs() <= 2.0 ** -14 + 2 * off + want.abs() * 2.0 ** -22).all())
