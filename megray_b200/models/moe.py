@@ -197,14 +197,16 @@ class MoELayer:
         sgd_step(self.w_down, self.g_down, self.cfg.lr)
 
     def train_step_device(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
+        """Returns this rank's share of the loss: the ranks' values add up to the loss that the gradients belong to, the
+        mean squared output over all ranks' tokens plus one balance loss over them (an n-th of it is in each value)."""
         y = self.forward(x, logits)
         loss, dy = mse_loss_grad(y, None, 1.0 / (self.cfg.tokens * self.n * self.cfg.hidden))
         self.backward(dy)
         self.optimizer_step()
-        return loss + self.balance_loss if self.cfg.balance_coef else loss
+        return loss + self.balance_loss / self.n if self.cfg.balance_coef else loss
 
     def train_step(self, x_host: torch.Tensor, logits_host: torch.Tensor) -> float:
-        """Public call: tokens and router logits come from pinned host memory, the loss goes back."""
+        """Public call: tokens and router logits come from pinned host memory, the loss goes back (this rank's share)."""
         self.x_dev.copy_(x_host, non_blocking=True)
         self.logits_dev.copy_(logits_host, non_blocking=True)
         return float(self.train_step_device(self.x_dev, self.logits_dev).item())

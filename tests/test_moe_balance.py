@@ -1,0 +1,45 @@
+"""The expert layer's balance loss in a training step: what several ranks' steps return, and what a step refuses."""
+import pytest
+import torch
+
+from megray_b200.models import MoEConfig
+from megray_b200.models import moe as module
+
+COEF, HIDDEN, EXPERTS, TOP = 0.3, 16, 4, 2
+
+
+class Rank(module.MoELayer):
+    """A layer on the CPU whose experts are the identity: one of ``n`` ranks with ``tokens`` tokens."""
+
+    def __init__(self, n, tokens, coef=COEF):
+        self.cfg = MoEConfig(experts=EXPERTS, hidden=HIDDEN, tokens=tokens, balance_coef=coef)
+        self.n, self.balance_loss = n, None
+
+    def forward(self, x, logits):
+        return x
+
+    def backward(self, dout):
+        self.dout = dout
+        if self.cfg.balance_coef:  # the loss over all ranks' tokens, the same on each
+            self.balance_loss = torch.tensor([self.cfg.balance_coef])
+
+    def optimizer_step(self):
+        pass
+
+
+@pytest.fixture
+def squares(monkeypatch):
+    """The squared error's definition for CPU tensors."""
+    monkeypatch.setattr(module, "mse_loss_grad", lambda y, target, scale: ((y * y).sum().view(1) * scale, 2 * scale * y))
+
+
+@pytest.mark.parametrize("coef", [COEF, 0.0])
+@pytest.mark.parametrize("n", [1, 2, 4])
+def test_returned_values_add_up_over_ranks_to_the_loss_that_is_differentiated(n, coef, squares):
+    x = torch.randn(8 * n, HIDDEN, generator=torch.Generator().manual_seed(n))
+    whole = Rank(1, 8 * n, coef)
+    want = whole.train_step_device(x, None)
+    ranks = [Rank(n, 8, coef) for _ in range(n)]
+    got = [rank.train_step_device(part, None) for rank, part in zip(ranks, x.chunk(n))]
+    torch.testing.assert_close(sum(got), want, rtol=1e-6, atol=0)
+    torch.testing.assert_close(torch.cat([rank.dout for rank in ranks]), whole.dout, rtol=1e-6, atol=0)
