@@ -131,7 +131,8 @@ class MoELayer:
 
     # ------------------------------------------------------------------ forward / backward
     def forward(self, x: torch.Tensor, logits: torch.Tensor) -> torch.Tensor:
-        self._logits = logits if self.cfg.balance_coef else None  # read again by the backward pass
+        # (the backward pass reads them again, and the caller may have overwritten them by then)
+        self._logits = logits.detach().clone() if self.cfg.balance_coef else None
         ep, F, H = self.ep, self.cfg.ffn, self.cfg.hidden
         px, pl = plain(x, (ep.T, H)), plain(logits, (ep.T, ep.E), torch.float32)
         args = self._native_forward_args() if px and pl else None

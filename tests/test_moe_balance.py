@@ -43,3 +43,17 @@ def test_returned_values_add_up_over_ranks_to_the_loss_that_is_differentiated(n,
     got = [rank.train_step_device(part, None) for rank, part in zip(ranks, x.chunk(n))]
     torch.testing.assert_close(sum(got), want, rtol=1e-6, atol=0)
     torch.testing.assert_close(torch.cat([rank.dout for rank in ranks]), whole.dout, rtol=1e-6, atol=0)
+
+
+@pytest.mark.gpu
+def test_logits_may_be_overwritten_between_the_passes():
+    cfg = MoEConfig(experts=8, hidden=256, ffn=128, tokens=300, capacity_factor=4.0, balance_coef=COEF)
+    layer = module.MoELayer(cfg)
+    x, dout = (torch.randn(300, 256, device="cuda").bfloat16() for _ in range(2))
+    logits = torch.randn(300, 8, device="cuda")
+    layer.forward(x, logits)
+    want = [t.clone() for t in layer.backward(dout)] + [layer.balance_loss, layer.expert_counts]
+    layer.forward(x, logits)
+    logits.copy_(torch.randn(300, 8, device="cuda"))
+    got = [*layer.backward(dout), layer.balance_loss, layer.expert_counts]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
