@@ -189,7 +189,12 @@ class MoELayer:
         return self.dx, self.dlogits
 
     def optimizer_step(self) -> None:
+        """One step over the expert weights.  The AdamW forms count their steps on the host, which a captured graph would
+        not do again: they refuse to be captured (``adamw_step`` takes the number as a tensor)."""
         if self.adamw is not None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("MoELayer.optimizer_step: a captured AdamW step would repeat this step's number; call "
+                                   "adamw_step on layer.adamw with the number in a tensor")
             self.steps += 1
             adamw_step([self.w_gu, self.w_down], [self.g_gu, self.g_down], self.adamw, self.cfg.lr, step=self.steps,
                        weight_decay=self.cfg.weight_decay)

@@ -57,3 +57,34 @@ def test_logits_may_be_overwritten_between_the_passes():
     logits.copy_(torch.randn(300, 8, device="cuda"))
     got = [*layer.backward(dout), layer.balance_loss, layer.expert_counts]
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_an_adamw_step_refuses_to_be_captured(monkeypatch):
+    """Its number is counted on the host: every replay would take the first one's bias correction."""
+    layer = Rank(1, 8)
+    layer.adamw, layer.steps = object(), 3
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError):
+        module.MoELayer.optimizer_step(layer)
+    assert layer.steps == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("optimizer", ["sgd", "adamw"])
+def test_steps_of_a_captured_layer(optimizer):
+    cfg = MoEConfig(experts=4, hidden=256, ffn=128, tokens=200, capacity_factor=4.0, balance_coef=COEF, optimizer=optimizer, lr=10.0 if optimizer == "sgd" else 1e-3)
+    layer = module.MoELayer(cfg)
+    x, logits = torch.randn(200, 256, device="cuda").bfloat16(), torch.randn(200, 4, device="cuda")
+    layer.train_step_device(x, logits)
+    graph = torch.cuda.CUDAGraph()
+    if optimizer == "adamw":
+        with pytest.raises(RuntimeError), torch.cuda.graph(graph):
+            layer.train_step_device(x, logits)
+        assert layer.steps == 1
+    else:
+        before = layer.w_gu.clone()
+        with torch.cuda.graph(graph):
+            layer.train_step_device(x, logits)
+        graph.replay()
+        assert not torch.equal(layer.w_gu, before)
+    assert bool(torch.isfinite(layer.train_step_device(x, logits)).all())
