@@ -84,8 +84,9 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
     p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v / (1 - b2^step)) + eps), all in float32.
 
     ``params`` are float32 or bf16, ``grads`` float32 or bf16 of the same sizes, in the order that ``state`` was made
-    with; a gradient that is None leaves its tensor and moments as they are.  ``copies`` (bf16, one per parameter, or
-    None) receive the updated parameters rounded.  ``step`` counts from 1.  ``lr``, ``step`` and ``grad_scale`` may be
+    with; a gradient that is None leaves its tensor and moments as they are.  ``copies``, when given, are as many bf16
+    tensors and receive the updated parameters rounded.  Parameters overlap neither one another nor anything else in the
+    call, and copies do not either: the tensors are worked on side by side.  ``step`` counts from 1.  ``lr``, ``step`` and ``grad_scale`` may be
     float32 tensors of one element on the device: a captured graph then follows their contents, while host numbers
     are part of the capture."""
     n = len(state.sizes)
@@ -137,9 +138,16 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
         return
     lib, stream = _lib.load(), raw_stream(device.index)
     pairs = {(params[0].dtype, grads[0].dtype)} if one_kind else set(zip(map(_dtype, params), map(_dtype, grads)))
+    if len(pairs) > 1:  # (a list of one kind is looked at by its call, before it launches anything)
+        for name, field in (("parameter", _P), ("copy", _COPY)):
+            places = [a for a, k in zip(records[:, field].tolist(), sizes) if a and k]
+            if len(set(places)) < len(places):
+                raise ValueError(f"adamw_step: a {name} is in the list twice")
     for pair in pairs:
         part = records if one_kind else records[[(p.dtype, g.dtype) == pair for p, g in zip(params, grads)]]
         args.p_dtype, args.g_dtype = _CODES[pair[0]], _CODES[pair[1]]
         rc = lib.megray_adamw(C.c_void_p(part.__array_interface__["data"][0]), len(part), args, stream)
+        if rc == -1:
+            raise ValueError("adamw_step: tensors of the list overlap or are not aligned to their elements")
         if rc != 0:
             raise RuntimeError(f"megray_adamw failed ({rc})")

@@ -28,7 +28,10 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <cmath>
+#include <memory>
+#include <new>
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -422,6 +425,41 @@ cudaError_t launch_typed(const Tensor* tensors, int count, int bits, const Args&
                      : launch_table<P, G, 32, 720>(tensors, count, a, stream);
 }
 
+// Whether ranges of `size` bytes an element overlap that `place` gives for the tensors: these would be written by
+// several CTAs at once.  Views of one buffer in their order take one look each, others are sorted.
+template <class F>
+cudaError_t refuse_overlap(const Tensor* tensors, int count, uint64_t size, F place) {
+    struct Range {
+        uint64_t begin, end;
+    };
+    auto range = [&](const Tensor& t) {
+        const uint64_t at = t.n != 0 ? reinterpret_cast<uintptr_t>(place(t)) : 0;
+        return Range{at, at != 0 ? at + t.n * size : 0};
+    };
+    uint64_t end = 0;
+    int i = 0;
+    for (; i < count; ++i) {
+        const Range r = range(tensors[i]);
+        if (r.begin == 0)
+            continue;
+        if (r.begin < end)
+            break;
+        end = r.end;
+    }
+    if (i == count)
+        return cudaSuccess;
+    const std::unique_ptr<Range[]> all(new (std::nothrow) Range[count]);
+    if (all == nullptr)
+        return cudaErrorMemoryAllocation;
+    for (int k = 0; k < count; ++k)
+        all[k] = range(tensors[k]);
+    std::sort(all.get(), all.get() + count, [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    for (int k = 1; k < count; ++k)
+        if (all[k].begin < all[k - 1].end)
+            return cudaErrorInvalidValue;
+    return cudaSuccess;
+}
+
 }  // namespace
 
 cudaError_t launch(const Tensor* tensors, int count, const Step& s, cudaStream_t stream) {
@@ -446,6 +484,11 @@ cudaError_t launch(const Tensor* tensors, int count, const Step& s, cudaStream_t
     if (s.m == nullptr || s.v == nullptr || (moments & 15) ||
         (s.bits == 8 && (s.m_scale == nullptr || s.v_scale == nullptr || (scales & 3))))
         return cudaErrorInvalidValue;
+    cudaError_t e = refuse_overlap(tensors, count, s.p_bf16 ? 2 : 4, [](const Tensor& t) { return t.p; });
+    if (e == cudaSuccess)
+        e = refuse_overlap(tensors, count, 2, [](const Tensor& t) { return t.copy; });
+    if (e != cudaSuccess)
+        return e;
     Args a{};
     a.m = s.m;
     a.v = s.v;

@@ -242,3 +242,37 @@ def test_bad_arguments_of_the_c_entry_are_refused_before_any_launch():
         assert lib.megray_adamw(rec, 1, _lib.AdamWArgs(**{**ok, **bad}), None) in (6, -1), bad
     for bad in ((0, 64, 0, 8, 0), (66, 64, 0, 8, 0), (64, 65, 0, 8, 0), (64, 64, 1, 8, 0)):
         assert lib.megray_adamw((_lib.C.c_uint64 * 5)(*bad), 1, _lib.AdamWArgs(**ok), None) == -1, bad
+
+
+@gpu
+def test_a_tensor_that_is_in_a_step_twice_is_refused():
+    from megray_b200.ops import adamw_step
+
+    params, grads, state = make([300, 300, 0, 0], torch.float32, torch.float32, 32)
+    copies = [torch.zeros(n, dtype=torch.bfloat16, device="cuda") for n in state.sizes]
+    before = params[0].clone()
+    flat = torch.zeros(500, device="cuda")
+    for bad in (dict(params=[params[0], params[0], *params[2:]]), dict(params=[flat[200:], flat[:300], *params[2:]]),
+                dict(copies=[copies[1], copies[1], *copies[2:]]),
+                dict(params=[params[0].bfloat16(), params[1], params[1][:0], params[1][:0]], copies=[copies[1], copies[1], *copies[2:]])):
+        kw = {**H, "params": params, "copies": copies, "step": 1, **bad}
+        with pytest.raises(ValueError):
+            adamw_step(kw.pop("params"), grads, state, kw.pop("lr"), **kw)
+    assert torch.equal(params[0], before) and not bool(state.m.any())
+    adamw_step(params, [grads[0], grads[0], *grads[2:]], state, step=1, copies=copies, **H)  # gradients are only read
+    assert not torch.equal(params[0], before)
+
+
+def test_overlapping_tensors_of_a_list_are_refused_by_the_c_entry():
+    from megray_b200 import _lib
+
+    lib = _lib.load()
+    # (addresses that are never read: the refusal comes before any launch)
+    args = _lib.AdamWArgs(p_dtype=7, g_dtype=7, bits=32, m=64, v=64, step=1.0)
+    step = lambda *recs: lib.megray_adamw((_lib.C.c_uint64 * (5 * len(recs)))(*sum(recs, ())), len(recs), args, None)  # noqa: E731
+    far, near, empty = (4096, 64, 0, 100, 0), (4096 - 399 * 4, 64, 0, 400, 1), (4096, 64, 0, 0, 3)
+    assert step(far, near) == -1 and step(near, far) == -1 and step(far, far) == -1
+    assert step(far, (1 << 20, 64, 0, 8, 2), near) == -1 and step((1 << 20, 64, 0, 8, 2), empty, near, far) == -1
+    copy = lambda p, at, n: (p, 64, at, n, 0)  # noqa: E731
+    assert step(copy(1 << 20, 4096, 100), copy(1 << 21, 4096 + 198, 100)) == -1
+    assert step(copy(1 << 20, 4096, 100), copy(1 << 21, 0, 8), copy(1 << 22, 4000, 100)) == -1
