@@ -60,17 +60,17 @@ def _problem(q, k, v, cu_seqlens, causal, scale):
     kv_heads, dtype, index = k.shape[1], q.dtype, q.get_device()
     if dim & 7 or not 8 <= dim <= 128 or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("attention: D is a multiple of 8 from 8 to 128, the query heads a multiple of the key heads")
-    if tokens >= 2 ** 31:
-        raise ValueError("attention: fewer than 2^31 rows")
+    if tokens >= 2 ** 31 - 512:
+        raise ValueError("attention: fewer than 2^31 - 512 rows")
     if scale is None:
         scale = 1.0 / math.sqrt(dim)
     elif not 0.0 < scale < math.inf:
         raise ValueError("attention: scale is positive")
     cu, seqs = None, 1
     if cu_seqlens is not None:
-        if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or
+        if (cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or not 2 <= cu_seqlens.numel() <= 2 ** 31 - 512 or
                 not cu_seqlens.is_contiguous() or cu_seqlens.get_device() != index):
-            raise ValueError("attention: cu_seqlens is a contiguous int32 tensor of at least 2 entries on q's device")
+            raise ValueError("attention: cu_seqlens is a contiguous int32 tensor of 2 to 2^31 - 512 entries on q's device")
         cu, seqs = cu_seqlens.data_ptr(), cu_seqlens.numel() - 1
     args = _lib.AttnArgs(cu, _CODES[dtype], tokens, heads, kv_heads, dim, seqs, 1 if causal else 0, scale,
                          gemm_error_flag(q.device).data_ptr())

@@ -1302,9 +1302,11 @@ bool bad(const Tensor& t) {
            t.row >= most || t.head >= most;
 }
 bool bad(const Problem& p) {
-    return p.tokens < 0 || p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads || p.dim < 8 || p.dim > kMaxDim || p.dim % 8 ||
-           p.seqs < 0 || (p.cu != nullptr && p.seqs < 1) || (reinterpret_cast<uintptr_t>(p.cu) & 3) || !(p.scale > 0.f) ||
-           !(p.scale < INFINITY);
+    // (tiles reach past the last row, and the search for one past the last sequence: their ends have to be numbers too)
+    constexpr int most = 0x7fffffff - 4 * TILE;
+    return p.tokens < 0 || p.tokens > most || p.heads < 1 || p.kv_heads < 1 || p.heads % p.kv_heads || p.dim < 8 ||
+           p.dim > kMaxDim || p.dim % 8 || p.seqs < 0 || p.seqs > most || (p.cu != nullptr && p.seqs < 1) ||
+           (reinterpret_cast<uintptr_t>(p.cu) & 3) || !(p.scale > 0.f) || !(p.scale < INFINITY);
 }
 // CTAs for the tiles of `rows` rows that find_tile numbers, `heads` for each; 0 when there are too many
 unsigned grid_for(const Problem& p, int rows, int heads) {

@@ -516,3 +516,12 @@ def test_finite_scores_of_any_size(first, dtype, size, scale, causal, sign):
     tol = val["out"].abs() * HALF[dtype] + weight["out"] * (HALF[dtype] + 2 * off + 2.0 ** -13) * 1.01 + (2.0 ** -24 if dtype == HF else 0.0)
     assert bool(((out.double() - val["out"]).abs() <= tol).all())
     assert bool(((lse.double() - want).abs() <= 2.0 ** -14 + 2 * off + want.abs() * 2.0 ** -22).all())
+
+
+def test_rows_and_sequences_whose_ends_would_pass_32_bits_are_refused():
+    from megray_b200 import _lib
+
+    size = lambda rows, seqs=1: _lib.load().megray_attention_bwd_workspace(  # noqa: E731
+        _lib.AttnArgs(cu=1024, dtype=10, tokens=rows, heads=1, kv_heads=1, dim=8, seqs=seqs, causal=1, scale=1.0))
+    assert size(2 ** 31 - 513) >= 4 * (2 ** 31 - 513)
+    assert size(2 ** 31 - 512) == 0 and size(2 ** 31 - 1) == 0 and size(8, 2 ** 31 - 1) == 0
