@@ -95,10 +95,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     Without ``cu_seqlens`` all rows are one prompt.  Rows behind the last prompt are not looked at and keep what
     ``out`` and ``lse`` hold there (zeros in tensors made here).  ``cu_seqlens`` is read on the device: it has to
     rise from 0 to at most T; nothing outside the tensors is touched if it does not, but rows may then go
-    unwritten.  Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32.  A NaN or
-    an infinity in the values of a prompt may reach any row of that prompt, those of other prompts and of rows
-    behind the last never do.  ``out`` may be ``q`` itself (the queries are then gone, also for the backward pass); beside
-    that neither result may overlap an input or the other."""
+    unwritten.
+
+    Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32; values beyond 2^90 may
+    overflow in them.  A query whose scores are all -infinity has the output NaN and the lse -infinity.  A NaN or an infinity
+    in the values of a prompt may reach any row of that prompt, those of other prompts and of rows behind the last never
+    do.  ``out`` may be ``q`` itself (the queries are then gone, also for the backward pass); beside that neither result may
+    overlap an input or the other."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention(q, k, v, cu_seqlens, causal=causal, scale=scale, out=out, lse=lse)
@@ -123,7 +126,13 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     same arguments.  Gradients of key / value heads are summed over the query heads that read them.  Given tensors
     are written to (any of the strides that the inputs may have, slices of one buffer among them); rows behind the
     last prompt are left as they are (zeros in tensors made here).  They may overlap neither the inputs, which are read
-    until the end, nor one another.  No atomics: the same inputs give the same bits."""
+    until the end, nor one another.  No atomics: the same inputs give the same bits.
+
+    Probabilities are formed anew from the scores and ``lse`` and are off by up to ``abs(lse) * 2^-20`` of themselves: with
+    scores (times scale) beyond some 1e4 gradients lose digits that the output keeps, and from 1e6 on they mean nothing.
+    Probabilities and score gradients are rounded to the type of ``q`` for their products.  Float16 has steps of 2^-24
+    below 6e-5 and ends at 65504: there ``dout`` is best scaled as losses are for that type, so that ``dout v`` over the
+    length of a prompt is well inside."""
     if isinstance(q, torch.Tensor) and q.is_cuda and q.get_device() != torch.cuda.current_device():
         with torch.cuda.device(q.device):
             return attention_bwd(dout, q, k, v, out, lse, cu_seqlens, causal=causal, scale=scale, dq=dq, dk=dk, dv=dv)

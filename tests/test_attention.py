@@ -525,3 +525,79 @@ def test_rows_and_sequences_whose_ends_would_pass_32_bits_are_refused():
         _lib.AttnArgs(cu=1024, dtype=10, tokens=rows, heads=1, kv_heads=1, dim=8, seqs=seqs, causal=1, scale=1.0))
     assert size(2 ** 31 - 513) >= 4 * (2 ** 31 - 513)
     assert size(2 ** 31 - 512) == 0 and size(2 ** 31 - 1) == 0 and size(8, 2 ** 31 - 1) == 0
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads", [(2, 2), (8, 1)])  # the second shares tiles between CTAs
+def test_nothing_is_written_outside_whatever_the_offsets(heads, kv_heads):
+    """Results in the middle of larger buffers: what lies around them, and the inputs, stay as they were."""
+    from megray_b200.ops import attention, attention_bwd, gemm_error_flag
+
+    rows, dim = 700, 64
+    q, k, v, do = make([rows], heads, kv_heads, dim, BF)
+    kept = [t.clone() for t in (q, k, v, do)]
+    def inside(h):
+        store = torch.full((rows + 512, h + 2, dim), 7.0, device="cuda", dtype=BF)
+        return store, store[256:256 + rows, 1:1 + h]
+    for bad in ([0, 300, 700], [-5, 100, 9000], [200, 100, 50], [0, 2 ** 31 - 1, -2 ** 31], [300, 400, 500], [900, 950, 1000],
+                [700, 700, 0, 700]):
+        cu = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        stores = [inside(h) for h in (heads, heads, kv_heads, kv_heads)]
+        lse = torch.full((heads + 2, rows), 7.0, device="cuda")
+        attention(q, k, v, cu, out=stores[0][1], lse=lse[1:1 + heads])
+        attention_bwd(do, q, k, v, stores[0][1], lse[1:1 + heads], cu, dq=stores[1][1], dk=stores[2][1], dv=stores[3][1])
+        torch.cuda.synchronize()
+        assert int(gemm_error_flag().item()) == 0
+        for store, view in stores:
+            view.fill_(7.0)
+            assert bool((store == 7.0).all()), bad
+        assert bool((lse[0] == 7.0).all()) and bool((lse[-1] == 7.0).all()), bad
+        assert all(torch.equal(a, b) for a, b in zip((q, k, v, do), kept)), bad
+
+
+@gpu
+@pytest.mark.parametrize("scale", [0.05, 0.3])
+@pytest.mark.parametrize("lengths,heads,kv_heads,dim,dtype", [([300, 77], 4, 2, 64, BF), ([1000, 30], 8, 1, 64, BF), ([500], 6, 2, 80, HF)])
+def test_gradients_at_other_scales(lengths, heads, kv_heads, dim, dtype, scale):
+    run_and_check(lengths, heads, kv_heads, dim, dtype, True, tail=3, scale=scale, seed=21)
+
+
+@gpu
+@pytest.mark.parametrize("lengths,heads,kv_heads,tail", [([300, 1, 77], 4, 2, 9), ([1000, 30], 8, 1, 0), ([0, 40, 0], 2, 2, 200)])
+def test_results_that_the_call_makes(lengths, heads, kv_heads, tail):
+    """Without given tensors: the same results, and zeros behind the last sequence."""
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make(lengths, heads, kv_heads, 64, BF, tail, seed=5)
+    n, cu = sum(lengths), ends(lengths)
+    for t in (q, k, v, do):
+        t[n:] = float("nan")
+    torch.full((1 << 22,), float("nan"), device="cuda")  # what a fresh tensor may hold
+    out, lse = attention(q, k, v, cu)
+    val, size, lse_want = reference(q, k, v, do, lengths, True)
+    check(out[:n], val["out"][:n], size["out"][:n], BF, "out")
+    assert bool(((lse[:, :n].double() - lse_want[:, :n]).abs() <= 2.0 ** -14).all())
+    assert not bool(out[n:].any()) and not bool(lse[:, n:].any())
+    for g, name in zip(attention_bwd(do, q, k, v, out, lse, cu), ("dq", "dk", "dv")):
+        check(g[:n], val[name][:n], size[name][:n], BF, name)
+        assert not bool(g[n:].any())
+
+
+@gpu
+@pytest.mark.parametrize("shift", [100.0, 3000.0, 20000.0])
+def test_gradients_of_scores_far_from_zero(shift):
+    """The backward pass takes probabilities from the scores and lse, both of about ``shift``: a score is four sums of
+    16 products, each cut or rounded to float32 (2^-23 of it), and the exponent is off by a half step of lse, of its
+    product with log2 e and of the scores' factor: below 2^-20 of ``shift`` in all."""
+    from megray_b200.ops import attention, attention_bwd
+
+    q, k, v, do = make([300], 2, 1, 64, BF, seed=9)
+    q[..., 0], k[..., 0] = 32.0, shift / 4 if shift < 1000 else 1024.0 * round(shift / 4096)
+    out, lse = attention(q, k, v)
+    val, size, lse_want = reference(q, k, v, do, [300], True)
+    far = float(lse_want.abs().max())
+    more = far * 2.0 ** -20
+    assert bool(((lse.double() - lse_want).abs() <= 2.0 ** -14 + more).all())
+    for g, name in zip((out, *attention_bwd(do, q, k, v, out, lse)), ("out", "dq", "dk", "dv")):
+        tol = val[name].abs() * HALF[BF] + size[name] * (HALF[BF] + 2.0 ** -13 + 2 * more) * 1.01
+        assert bool(((g.double() - val[name]).abs() <= tol).all()), name
