@@ -10,10 +10,12 @@
 // kept between steps is rounded.  A NaN or an infinity in a block's gradients makes the block's scale NaN or
 // infinite and with it the block.
 //
-// Moments are formed with every operation rounded on its own, in the order of the formulas (no contraction into fused
+// m and v are formed with every operation rounded on its own, in the order of the formulas (no contraction into fused
 // multiply-adds): they are those of a list of elementary float32 operations bit for bit, so that an
-// 8-bit moment next to the border of two numbers falls to the same side everywhere.  The update itself, which is not
-// kept in 8 bits, uses the hardware's approximate reciprocal, a few float32 steps off.
+// 8-bit m next to the border of two numbers falls to the same side everywhere.  The root that 8-bit moments keep is up to
+// one float32 step off the rounded one, and which of two ways it is found goes by all eight numbers of a lane: the same
+// blocks give the same bits however a list is split, the same number among others may not.  The update itself uses the
+// hardware's approximate reciprocal, a few float32 steps off.
 //
 // Bound by HBM, with the issue slots close behind: 10 bytes an element with 8-bit moments and bf16 tensors leave
 // about 55 instructions for it; products and sums are issued in pairs.  A warp takes blocks of 256 elements, two

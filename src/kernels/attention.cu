@@ -356,7 +356,7 @@ __device__ __forceinline__ void store_sums(uint32_t taddr, int from, int to, flo
 // A CTA takes two tiles of 128 queries of one head and walks over the keys once; while one warpgroup works on the
 // scores of its tile, a row a thread, the tensor cores work for the other tile.  P lies over the scores that it comes
 // from.  Bound by that chain: 3400 cycles for two tiles whose products take 2230.  (16384 tokens, 8 heads of 128,
-// causal: 452 us, 1.22 PFLOP/s.) The running maximum is that of the first block until a later one is more than 2^32
+// causal: 451 us, 1.22 PFLOP/s, in a short run at full clocks; 503 us at the power limit.)  The running maximum is that of the first block until a later one is more than 2^32
 // larger (2^8 for float16, whose numbers end at 2^16): P may then be that large, which changes nothing in its relative
 // precision.  So a block's exponentials do not wait for its maximum, which is found beside them; only if it did rise
 // that far they are taken again, and the threads that own its rows rescale the accumulator in TMEM.
@@ -935,14 +935,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
 // ================================================================ backward: dK and dV
 //
 // A CTA takes 128 keys of one key / value head and walks over the queries of every head of its group; rows of the
-// score tiles are keys, so P^T and dS^T are left operands as they stand.
+// score tiles are keys, so P^T and dS^T are left operands as they stand.  Where there are few tiles of keys, several CTAs
+// share the queries of one and leave float32 sums that a last kernel adds up in order.
 // Scores and their gradients take turns in one region of TMEM, A; probabilities and score gradients as 16-bit operands
 // lie in another, B, so that neither waits for the product that reads the other:
-// Where there are few tiles of keys, several CTAs share the queries of one and leave float32 sums that a last kernel
-// adds up in order.
 //   tensor cores:  dV += P^T(i-1) dO, A = dP^T(i), dK += dS^T(i-1) Q, A = S^T(i+1), ...
 //   row warps:     P(i) from S(i) (in registers: A is free at once)    dS(i) from dP(i)
 // (P written over S and dS over dP, so that S(i+1) waited for dV: 3180 cycles an iteration; the products take 2048.)
+// The compiler keeps 24 bytes of a thread of this kernel in local memory.
 template <int DP, bool FP16>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
         dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -1402,10 +1402,11 @@ cudaError_t launch_forward(const Problem& p, Tensor q, Tensor k, Tensor v, Tenso
 
 // CTAs that share one tile of keys.  A tile takes the heads of its group one after the other, so that with grouped heads
 // few tiles mean long ones: then about two CTAs a processor, but no more than the group has heads (dQ runs beside and
-// has as long to go for one head).  4096 tokens, 4 heads of one group: 198 us unshared, 114 by two, 99 by ten; 2048
-// tokens, 16 heads in 2 groups: 203, 118 and 88.  Without groups sharing only costs (1000 tokens, 8 heads: 17 us
-// unshared, 25 by two), and so it does where there is a CTA for every processor (5003 tokens, 12 heads in 4 groups: 137
-// and 160).
+// has as long to go for one head).  The whole backward pass on the device: 4096 tokens, 4 heads of 128 in one group, causal:
+// 196 us unshared, 111 by two, 66 by four as chosen; 2048 tokens, 16 heads in 2 groups: 202, 115 and, by eight as
+// chosen, 78 (by four 70).  Without groups sharing only costs (1000 tokens, 8 heads of 64: 20 us unshared, 23 by two),
+// and so it does where there is a CTA for every processor (5003 tokens, 12 heads of 80 in 4 groups, all keys: 359 to
+// 390 unshared, 403 by two).
 static int splits_for(const Problem& p) {
     const int64_t seqs = p.cu != nullptr ? p.seqs : 1, group = p.heads / p.kv_heads;
     // (where the sequences end is not known here: half a tile is taken to be empty in each)
