@@ -209,8 +209,8 @@ size_t megray_attention_bwd_workspace(const megray_attn_args* a);  /* 0 for argu
 /* AdamW over a list of tensors.  `block` is the tensor's first block of 256 elements in the moment buffers,
  * which cover whole blocks.  bits = 32: m and v are float32; bits = 8: m and v hold e4m3 numbers of m and of
  * sqrt(v), the scales one float32 per block.  Parameters do not overlap, nor do copies (a list in which they do
- * is refused), nor either anything else in the call.  The *_dev pointers, where not null, name one float32 on the device each
- * that takes the place of the host value (a captured graph then follows them). */
+ * is refused), nor either anything else in the call.  The *_dev pointers, where not null, name one float32 on the
+ * device each that takes the place of the host value (a captured graph then follows them). */
 typedef struct {
     void* p;
     const void* g;

@@ -86,9 +86,9 @@ def adamw_step(params, grads, state: AdamWState, lr, *, step, betas=(0.9, 0.999)
     ``params`` are float32 or bf16, ``grads`` float32 or bf16 of the same sizes, in the order that ``state`` was made
     with; a gradient that is None leaves its tensor and moments as they are.  ``copies``, when given, are as many bf16
     tensors and receive the updated parameters rounded.  Parameters overlap neither one another nor anything else in the
-    call, and copies do not either: the tensors are worked on side by side.  ``step`` counts from 1.  ``lr``, ``step`` and ``grad_scale`` may be
-    float32 tensors of one element on the device: a captured graph then follows their contents, while host numbers
-    are part of the capture."""
+    call, and copies do not either: the tensors are worked on side by side.  ``step`` counts from 1.  ``lr``, ``step`` and
+    ``grad_scale`` may be float32 tensors of one element on the device: a captured graph then follows their contents,
+    while host numbers are part of the capture."""
     n = len(state.sizes)
     params, grads, copies = list(params), list(grads), None if copies is None else list(copies)
     if len(params) != n or len(grads) != n or (copies is not None and len(copies) != n):

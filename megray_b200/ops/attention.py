@@ -97,8 +97,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: tor
     rise from 0 to at most T; nothing outside the tensors is touched if it does not, but rows may then go
     unwritten.
 
-    Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32; values beyond 2^90 may
-    overflow in them.  A query whose scores are all -infinity has the output NaN and the lse -infinity.  A NaN or an infinity
+    Probabilities are rounded to the type of ``v`` for the product with it, all sums are float32; values beyond 2^75 may
+    overflow in them (a probability counts up to 2^32 there).  A query whose scores are all -infinity has the output NaN and the lse -infinity.  A NaN or an infinity
     in the values of a prompt may reach any row of that prompt, those of other prompts and of rows behind the last never
     do.  ``out`` may be ``q`` itself (the queries are then gone, also for the backward pass); beside that neither result may
     overlap an input or the other."""

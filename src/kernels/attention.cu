@@ -356,10 +356,11 @@ __device__ __forceinline__ void store_sums(uint32_t taddr, int from, int to, flo
 // A CTA takes two tiles of 128 queries of one head and walks over the keys once; while one warpgroup works on the
 // scores of its tile, a row a thread, the tensor cores work for the other tile.  P lies over the scores that it comes
 // from.  Bound by that chain: 3400 cycles for two tiles whose products take 2230.  (16384 tokens, 8 heads of 128,
-// causal: 451 us, 1.22 PFLOP/s, in a short run at full clocks; 503 us at the power limit.)  The running maximum is that of the first block until a later one is more than 2^32
-// larger (2^8 for float16, whose numbers end at 2^16): P may then be that large, which changes nothing in its relative
-// precision.  So a block's exponentials do not wait for its maximum, which is found beside them; only if it did rise
-// that far they are taken again, and the threads that own its rows rescale the accumulator in TMEM.
+// causal: 451 us, 1.22 PFLOP/s, in a short run at full clocks; 503 us at the power limit.)
+// The running maximum is that of the first block until a later one is more than 2^32 larger (2^8 for float16, whose
+// numbers end at 2^16): P may then be that large, which changes nothing in its relative precision.  So a block's
+// exponentials do not wait for its maximum, which is found beside them; only if it did rise that far they are taken
+// again, and the threads that own its rows rescale the accumulator in TMEM.
 constexpr int FWD_ROW_WARPS = 8, FWD_MMA = 8, FWD_TMA = 9;  // (and two warps that idle)
 constexpr int FWD_THREADS = 32 * (FWD_ROW_WARPS + 4);
 constexpr int FWD_STAGES = 4;
